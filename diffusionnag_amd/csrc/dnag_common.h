@@ -345,6 +345,17 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
     return r;
 }
 
+// `v` rounded to fp32 before anything else is done with it.  A hi/lo fp16 split of a product needs it: without it the
+// compiler may fold the product into the conversion for hi (v_fma_mixlo_f16, one rounding) and convert the rounded product
+// where hi is subtracted for lo.  Next to a tie the two hi differ by an fp16 step and the pair is 2^-11 off: a few values
+// in ten thousand, a score 1e-5 off instead of 1e-6.  (A product with a power of two is exact and cannot differ.)
+__host__ __device__ __forceinline__ float whole(float v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm("" : "+v"(v));
+#endif
+    return v;
+}
+
 __device__ __forceinline__ float elu1(float x) { return x > 0.f ? x : expm1f(x); }
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + expf(-x)); }
 

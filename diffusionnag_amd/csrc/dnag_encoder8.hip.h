@@ -11,8 +11,8 @@
 //   P0  finish the row statistics of h (see below): concat slice of the previous layer (output norm, transformer.py:177)
 //       and LN1(h) -> A16, from the wave's registers
 //   P1  q|k|v = A16 Wqkv'^T + b            (3 tile jobs per wave)                    -> qkv fp32 [64][192]
-//   P2  attention: one thread per (graph, head, query pair): K and V rows are read once for two queries (scalar pairs that
-//       the compiler packs into v_pk_fma_f32 where it can); 20 keys: two blocks with a running maximum   -> A16 (scale sa_o)
+//   P2  attention: one thread per (graph, head, query pair): K and V rows are read once for two queries (scalar
+//       pairs); 20 keys: two blocks with a running maximum   -> A16 (scale sa_o)
 //   P3  h += A16 Wo^T + bo                 (the wave's tile of h lives in registers)
 //   P4  LN2(h) -> A16, from the wave's registers
 //   P5  hidden = relu(A16 W1'^T + b1'), MFMA operands swapped so that a lane owns one batch row and writes its 16
@@ -34,12 +34,8 @@
 #include "dnag_encoder.hip.h"
 #include <type_traits>
 
-// Two queries per thread as scalar pairs; the compiler's SLP pass turns most of these pairs into v_pk_fma_f32 /
-// v_pk_mul_f32 / v_pk_add_f32 with op_sel broadcasts on its own (244 packed instructions in the production ISA).
-// Round 2 also carried a hand-packed variant (float2 ext vectors, -DENC8_PK) that was bit-exact at one workgroup per CU
-// and wrong in lanes 32-63 at two; its ISA was diffed against this build in round 3 (profiles/r03_enc8_pk_isa.md: same
-// barriers, waits and register budget, no spills; it differs in which softmax steps ride on packed adds behind
-// v_exp_f32 / v_rcp_f32 results), no cause could be named from the ISA, and the variant was deleted.
+// Two queries per thread as scalar pairs (the library is built without packed fp32 instructions, see the Makefile: a
+// hand-packed variant of this phase was bit-exact at one workgroup per CU and wrong in lanes 32-63 at two).
 struct v2f {
     float x, y;
     __device__ __forceinline__ v2f operator*(v2f o) const { return v2f{x * o.x, y * o.y}; }
@@ -68,9 +64,9 @@ struct Enc8Geom {
 __device__ __forceinline__ void split4(const v4f v, h4 &hi, h4 &lo) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const _Float16 x = (_Float16)v[e];
+        const _Float16 x = (_Float16)whole(v[e]);
         hi[e] = x;
-        lo[e] = (_Float16)(v[e] - (float)x);
+        lo[e] = (_Float16)whole(v[e] - (float)x);
     }
 }
 

@@ -1001,12 +1001,9 @@ static int side_for_current_device(SideStream **out) {
     std::lock_guard<std::mutex> lk(g_side_mu);
     SideStream &s = g_side[dev];
     if (!s.ok) {
-        // highest priority: the surrogate's many short, under-filled kernels are dispatched as they become ready and the
-        // score network's large ones take what is left (OFA, B = 4096, same box: 657 samples/s on one stream, 683 with
-        // this stream at the lowest priority, 720 at the default, 734 at the highest)
-        int lo = 0, hi = 0;
-        HIP_TRY(hipDeviceGetStreamPriorityRange(&lo, &hi));
-        HIP_TRY(hipStreamCreateWithPriority(&s.st, hipStreamNonBlocking, hi));
+        // default priority, like every stream of the process: work on streams of different priorities can end up waiting for
+        // good on this driver (OFA, B = 4096, same box: 657 samples/s on one stream, 720 with this one)
+        HIP_TRY(hipStreamCreateWithFlags(&s.st, hipStreamNonBlocking));
         // no system-scope fence at the events: both streams are on this device (a record costs 4.8 instead of 6.4 us on the
         // recording stream; NB201 2794 -> 2809 samples/s same box)
         HIP_TRY(hipEventCreateWithFlags(&s.fork, hipEventDisableTiming | hipEventDisableSystemFence));
