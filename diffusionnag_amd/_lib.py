@@ -34,6 +34,10 @@ EXPORTS = (
     "dnag_train_workspace_bytes", "dnag_dropout_mask_bytes", "dnag_dropout_fill", "dnag_cate_dsm_step",
     "dnag_pred_forward_grad_noalloc", "dnag_optim_workspace_bytes", "dnag_optim_args_bytes", "dnag_optim_step",
     "dnag_langevin_partials_floats", "dnag_pred_workspace_bytes",
+    "dnag_embed_forward", "dnag_embed_grad_workspace_bytes", "dnag_embed_grad",
+    "dnag_block_norms_args_bytes", "dnag_block_norms_grad_workspace_bytes", "dnag_block_norms_forward", "dnag_block_norms_grad",
+    "dnag_distill_args_bytes", "dnag_distill_workspace_bytes", "dnag_distill_loss", "dnag_distill_loss_grad", "dnag_distill_backward",
+    "dnag_sample_args_bytes", "dnag_sample_tokens",
 )
 
 
@@ -105,6 +109,32 @@ class OptimArgsC(C.Structure):
 
 
 OPTIM_ADAM, OPTIM_EMA = 1, 2
+F32, BF16, F16 = 0, 1, 2
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+
+
+class BlockNormsArgsC(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "dim", "gate_rows")] +
+                [(n, C.c_int32) for n in ("dtype", "x_dtype", "layer_norm", "pre", "small_f32")] +
+                [("residual_scale", C.c_float), ("eps", C.c_float)] +
+                [(n, C.c_void_p) for n in ("x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias")] +
+                [("x_stride", C.c_int64), ("y_stride", C.c_int64)] + [(n, C.c_void_p) for n in ("x_new", "h", "grad_x", "grad_h")] +
+                [("grad_x_stride", C.c_int64), ("grad_h_stride", C.c_int64)] +
+                [(n, C.c_void_p) for n in ("dx", "dy", "d_gate", "d_post_weight", "d_post_bias", "d_pre_weight", "d_pre_bias", "workspace")] +
+                [("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)])
+
+
+class DistillArgsC(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "vocab", "logits_stride")] +
+                [(n, C.c_int32) for n in ("k", "dtype", "teacher_dtype", "ids_bytes", "reduction")] + [("temperature", C.c_float)] +
+                [(n, C.c_void_p) for n in ("logits", "teacher_ids", "teacher_logits", "row_weight", "loss", "stats", "grad_out", "grad", "workspace")] +
+                [("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)])
+
+
+class SampleArgsC(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "vocab", "logits_stride")] + [("dtype", C.c_int32), ("top_k", C.c_int32)] +
+                [(n, C.c_double) for n in ("temperature", "top_p", "min_p")] +
+                [(n, C.c_void_p) for n in ("logits", "u", "temperature_rows", "top_k_rows", "top_p_rows", "min_p_rows", "out", "stream")])
 
 _lib: Optional[C.CDLL] = None
 
@@ -193,6 +223,26 @@ def load() -> C.CDLL:
     if lib.dnag_pc_args_bytes() != C.sizeof(PcArgsC) or lib.dnag_train_args_bytes() != C.sizeof(TrainArgsC):
         raise ImportError(f"{LIB_PATH}: argument structs ({lib.dnag_pc_args_bytes()}, {lib.dnag_train_args_bytes()} bytes) do not "
                           f"match this binding ({C.sizeof(PcArgsC)}, {C.sizeof(TrainArgsC)}); rebuild the library")
+    i64, f32 = C.c_int64, C.c_float
+    lib.dnag_embed_forward.restype = i32
+    lib.dnag_embed_forward.argtypes = [vp, i32, i64, vp, i64, i64, i64, i32, f32, vp, vp]
+    lib.dnag_embed_grad_workspace_bytes.restype = sz
+    lib.dnag_embed_grad_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.dnag_embed_grad.restype = i32
+    lib.dnag_embed_grad.argtypes = [vp, i32, i64, vp, i64, i64, i64, i32, f32, i64, vp, vp, sz, vp]
+    for struct, size, workspace, calls in (
+            (BlockNormsArgsC, "dnag_block_norms_args_bytes", "dnag_block_norms_grad_workspace_bytes", ("dnag_block_norms_forward", "dnag_block_norms_grad")),
+            (DistillArgsC, "dnag_distill_args_bytes", "dnag_distill_workspace_bytes", ("dnag_distill_loss", "dnag_distill_loss_grad", "dnag_distill_backward")),
+            (SampleArgsC, "dnag_sample_args_bytes", None, ("dnag_sample_tokens",))):
+        getattr(lib, size).restype = sz
+        if getattr(lib, size)() != C.sizeof(struct):
+            raise ImportError(f"{LIB_PATH}: {size}() is {getattr(lib, size)()}, this binding has {C.sizeof(struct)}; rebuild the library")
+        if workspace:
+            getattr(lib, workspace).restype = sz
+            getattr(lib, workspace).argtypes = [C.POINTER(struct)]
+        for call in calls:
+            getattr(lib, call).restype = i32
+            getattr(lib, call).argtypes = [C.POINTER(struct)]
     _lib = lib
     return lib
 

@@ -1,0 +1,437 @@
+// The seam between two blocks of a network: the norm behind a block with the block's gate and the residual scale, and the
+// norm in front of the next block, in one pass over the rows.
+//   forward:   x' = rs x + g N_post(y),   h = N_pre(x')          (y == NULL: h = N_pre(x), the entry of the first block)
+//   N is RMSNorm (v / rms(v) w) or LayerNorm ((v - mean) / std w + b); g is one row for every `rows_per_gate` rows.
+//   backward:  with a = dh w_pre, xhat = (x' - mean) r:   d = dx' + r (a - [mean a] - xhat mean(a xhat)),   dx = rs d,
+//              dg += d n,  b = d g w_post,  dy = r_y (b - [mean b] - yhat mean(b yhat)),  dw += rows' sums    ([.]: LayerNorm)
+//   The backward pass reads x and y again and recomputes x' in fp32: as many bytes as reading a saved x', without its rounding.
+// Bound by HBM: four rows per row forward, six or seven backward.  A team of TPR lanes holds a row in registers, eight
+// columns per lane (and twice that above 8192 columns), so every value is read once; statistics are fp32 and two-pass
+// (mean first) for LayerNorm.  Gradients of the weights and of shared gates are summed by every block over its own rows in
+// registers, then over blocks in block order by a second launch: no atomics, the same bits every time.
+#include "dnag_token_common.h"
+
+struct BnArgs {
+    const void *x, *y, *gate, *pw, *pb, *qw, *qb;      // q*: the norm in front (pre), p*: the norm behind (post)
+    void *xn, *h;
+    const void *gx, *gh;                               // backward: gradients of xn and h
+    void *dx, *dy, *dgate;
+    float *part, *gpart;                               // backward: [blocks][arrays][d], [G][S][d]
+    int64_t xs, ys, gxs, ghs;                          // row strides in elements
+    int64_t rows, rpg, G;                              // rows per gate row, gate rows
+    int64_t split_rows;                                // backward: rows of one work item (a gate row has S items)
+    int S, d, pre, small32;                            // small32: bit 0 gate, bit 1 post norm, bit 2 pre norm are fp32
+    float rs, eps, inv_d;
+};
+
+template <int TPR> struct RowSum {
+    float (*red)[16];
+    int turn = 0;
+    __device__ __forceinline__ float operator()(float v) {
+        if constexpr (TPR <= 64) return team_sum<TPR>(v);
+        v = team_sum<64>(v);
+        float *b = red[turn];
+        turn ^= 1;                                     // two buffers: the one being read is written again a barrier later
+        if ((threadIdx.x & 63) == 0) b[threadIdx.x >> 6] = v;
+        __syncthreads();
+        float s = b[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) s += b[w];
+        return s;
+    }
+};
+
+// v -> (v - mean) r in place; r returned.  Columns past d hold zeros and stay zeros.
+template <bool LN, int NV, class Sum>
+__device__ __forceinline__ float normalise(f8 (&v)[NV], const int (&n)[NV], Sum &sum, float eps, float inv_d) {
+    if constexpr (LN) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) s += sum8(v[j]);
+        const float mean = sum(s) * inv_d;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = e < n[j] ? v[j][e] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) q += sum8(v[j] * v[j]);
+    const float r = 1.0f / sqrtf(sum(q) * inv_d + eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] *= r;
+    return r;
+}
+
+template <class TX, class TY, int TPR, int NV, bool LN>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_kernel(const BnArgs a) {
+    constexpr int NT = TPR <= 64 ? 256 / TPR : 1;
+    __shared__ float red[2][16];
+    RowSum<TPR> sum{red};
+    const int lane = threadIdx.x & (TPR - 1);
+    const int64_t row = (int64_t)blockIdx.x * NT + threadIdx.x / TPR;
+    if (row >= a.rows) return;                         // whole teams; TPR > 64: the block has one team
+    int n[NV];
+    f8 x[NV], y[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + lane) * 8;
+        n[j] = a.d - c;
+        x[j] = y[j] = splat8(0.f);
+        if (n[j] > 0) {
+            x[j] = load8_n((const TX *)a.x + row * a.xs + c, n[j]);
+            if (a.y) y[j] = load8_n((const TY *)a.y + row * a.ys + c, n[j]);
+        }
+    }
+    if (a.y) {
+        normalise<LN>(y, n, sum, a.eps, a.inv_d);
+        const size_t g0 = (size_t)(row / a.rpg) * a.d;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * TPR + lane) * 8;
+            if (n[j] <= 0) continue;
+            f8 v = y[j];
+            if (a.pw) v *= load8_either<TY>(a.pw, a.small32 & 2, c, n[j]);
+            if (LN && a.pb) v += load8_either<TY>(a.pb, a.small32 & 2, c, n[j]);
+            if (a.gate) v *= load8_either<TY>(a.gate, a.small32 & 1, g0 + c, n[j]);
+            x[j] = x[j] * a.rs + v;
+            store8_n((TX *)a.xn + row * a.d + c, x[j], n[j]);
+        }
+    }
+    if (!a.pre) return;
+    normalise<LN>(x, n, sum, a.eps, a.inv_d);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + lane) * 8;
+        if (n[j] <= 0) continue;
+        f8 v = x[j];
+        if (a.qw) v *= load8_either<TY>(a.qw, a.small32 & 4, c, n[j]);
+        if (LN && a.qb) v += load8_either<TY>(a.qb, a.small32 & 4, c, n[j]);
+        store8_n((TY *)a.h + row * a.d + c, v, n[j]);
+    }
+}
+
+// order of the partial sums: pre weight, post weight, pre bias, post bias (the biases for LayerNorm only)
+template <class TX, class TY, int TPR, int NV, bool LN>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel(const BnArgs a) {
+    constexpr int NT = TPR <= 64 ? 256 / TPR : 1, NA = LN ? 4 : 2;
+    __shared__ float red[2][16];
+    __shared__ float comb[NT > 1 ? 256 * 8 * NV : 1];
+    RowSum<TPR> sum{red};
+    const int lane = threadIdx.x & (TPR - 1), team = threadIdx.x / TPR;
+    int n[NV];
+    f8 acc[NA][NV], dg[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        n[j] = a.d - (j * TPR + lane) * 8;
+#pragma unroll
+        for (int k = 0; k < NA; ++k) acc[k][j] = splat8(0.f);
+    }
+    auto one_row = [&](int64_t row, size_t g0) {
+        f8 x[NV], y[NV], gx[NV], gh[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * TPR + lane) * 8;
+            x[j] = y[j] = gx[j] = gh[j] = splat8(0.f);
+            if (n[j] > 0) {
+                x[j] = load8_n((const TX *)a.x + row * a.xs + c, n[j]);
+                if (a.y) y[j] = load8_n((const TY *)a.y + row * a.ys + c, n[j]);
+                if (a.gx) gx[j] = load8_n((const TX *)a.gx + row * a.gxs + c, n[j]);
+                if (a.gh) gh[j] = load8_n((const TY *)a.gh + row * a.ghs + c, n[j]);
+            }
+        }
+        auto small = [&](const void *p, int bit, size_t at, int j, float none) {
+            return p && n[j] > 0 ? load8_either<TY>(p, a.small32 & bit, at, n[j]) : splat8(none);
+        };
+        float ry = 0.f;
+        if (a.y) {
+            ry = normalise<LN>(y, n, sum, a.eps, a.inv_d);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * TPR + lane) * 8;
+                f8 v = y[j] * small(a.pw, 2, c, j, 1.f);
+                if (LN) v += small(a.pb, 2, c, j, 0.f);
+                x[j] = x[j] * a.rs + v * small(a.gate, 1, g0 + c, j, 1.f);
+            }
+        }
+        if (a.pre) {
+            const float r = normalise<LN>(x, n, sum, a.eps, a.inv_d);
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                acc[0][j] += gh[j] * x[j];
+                if constexpr (LN) acc[2][j] += gh[j];
+                gh[j] *= small(a.qw, 4, (j * TPR + lane) * 8, j, 1.f);
+                s1 += sum8(gh[j] * x[j]);
+                if (LN) s2 += sum8(gh[j]);
+            }
+            s1 = sum(s1) * a.inv_d;
+            if (LN) s2 = sum(s2) * a.inv_d;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) gx[j] += (gh[j] - s2 - x[j] * s1) * r;
+        }
+        const float back = a.y ? a.rs : 1.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (n[j] > 0) store8_n((TX *)a.dx + row * a.d + (j * TPR + lane) * 8, gx[j] * back, n[j]);
+        if (!a.y) return;
+        float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * TPR + lane) * 8;
+            const f8 w = small(a.pw, 2, c, j, 1.f);
+            f8 v = y[j] * w;
+            if (LN) v += small(a.pb, 2, c, j, 0.f);
+            dg[j] += gx[j] * v;
+            gx[j] *= small(a.gate, 1, g0 + c, j, 1.f);
+            if (n[j] < 8)                              // columns past d carry the LayerNorm means of gx: nothing of them is summed
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (e >= n[j]) gx[j][e] = 0.f;
+            acc[1][j] += gx[j] * y[j];
+            if constexpr (LN) acc[3][j] += gx[j];
+            gx[j] *= w;
+            t1 += sum8(gx[j] * y[j]);
+            if (LN) t2 += sum8(gx[j]);
+        }
+        t1 = sum(t1) * a.inv_d;
+        if (LN) t2 = sum(t2) * a.inv_d;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (n[j] > 0) store8_n((TY *)a.dy + row * a.d + (j * TPR + lane) * 8, (gx[j] - t2 - y[j] * t1) * ry, n[j]);
+    };
+    // adds the teams' registers in team order; the sum is valid in team 0
+    auto join_teams = [&](f8 (&v)[NV]) {
+        if constexpr (NT > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NV; ++j) *(f8 *)(comb + (size_t)(j * 256 + threadIdx.x) * 8) = v[j];
+            __syncthreads();
+            if (team == 0)
+                for (int t = 1; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) v[j] += *(const f8 *)(comb + (size_t)(j * 256 + t * TPR + lane) * 8);
+        }
+    };
+    auto clear = [&]() {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) dg[j] = splat8(0.f);
+    };
+    auto put_gate = [&](int64_t g, int s) {
+        if (!a.dgate) return;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * TPR + lane) * 8;
+            if (n[j] <= 0) continue;
+            if (a.S == 1) store8_either<TY>(a.dgate, a.small32 & 1, (size_t)g * a.d + c, dg[j], n[j]);
+            else store8_n(a.gpart + ((size_t)g * a.S + s) * a.d + c, dg[j], n[j]);
+        }
+    };
+    if (NT > 1 && a.rpg < NT) {                        // short runs of rows per gate: one team takes a run
+        for (int64_t g = (int64_t)blockIdx.x * NT + team; g < a.G; g += (int64_t)gridDim.x * NT) {
+            clear();
+            for (int64_t r = g * a.rpg; r < (g + 1) * a.rpg; ++r) one_row(r, (size_t)g * a.d);
+            put_gate(g, 0);
+        }
+    } else {                                           // the block takes `split_rows` rows of one gate row at a time
+        for (int64_t w = blockIdx.x; w < a.G * a.S; w += gridDim.x) {
+            const int64_t g = w / a.S;
+            const int s = (int)(w - g * a.S);
+            const int64_t r0 = g * a.rpg + s * a.split_rows, end = (g + 1) * a.rpg, r1 = r0 + a.split_rows < end ? r0 + a.split_rows : end;
+            clear();
+            for (int64_t r = r0 + team; r < r1; r += NT) one_row(r, (size_t)g * a.d);
+            if (a.dgate) {
+                join_teams(dg);
+                if (team == 0) put_gate(g, s);
+            }
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int k = 0; k < NA; ++k) {
+        join_teams(acc[k]);
+        if (team == 0)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (n[j] > 0) store8_n(a.part + ((size_t)blockIdx.x * NA + k) * a.d + (j * TPR + lane) * 8, acc[k][j], n[j]);
+    }
+}
+
+// sums over the blocks' (weights) or a gate row's pieces: sixteen waves add a contiguous share each, then in wave order
+struct BnJoin {
+    const float *part, *gpart;
+    void *out[4];
+    void *dgate;
+    int na, nblk, S, d, small32;
+};
+template <class TY> __device__ __forceinline__ void put1(void *p, bool f32, size_t at, float v) {
+    if (f32) ((float *)p)[at] = v;
+    else ((TY *)p)[at] = (TY)v;
+}
+template <class TY>
+__global__ __launch_bounds__(1024) void block_norms_join_kernel(const BnJoin a) {
+    __shared__ float q[16][64];
+    const int col = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + col;
+    const bool weight = (int)blockIdx.y < a.na;
+    const int g = (int)blockIdx.y - a.na;
+    if (weight && !a.out[blockIdx.y]) return;
+    const int count = weight ? a.nblk : a.S;
+    const float *src = weight ? a.part + (size_t)blockIdx.y * a.d : a.gpart + (size_t)g * a.S * a.d;
+    const size_t step = weight ? (size_t)a.na * a.d : (size_t)a.d;
+    const int per = (count + 15) / 16, k0 = w * per, k1 = k0 + per < count ? k0 + per : count;
+    float s = 0.f;
+    if (c < a.d)
+#pragma unroll 8
+        for (int k = k0; k < k1; ++k) s += src[k * step + c];
+    q[w][col] = s;
+    __syncthreads();
+    if (w != 0 || c >= a.d) return;
+    s = q[0][col];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += q[k][col];
+    if (weight) put1<TY>(a.out[blockIdx.y], a.small32 & ((blockIdx.y & 1) ? 2 : 4), c, s);
+    else put1<TY>(a.dgate, a.small32 & 1, (size_t)g * a.d + c, s);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+namespace {
+constexpr int BN_MAX_D = 16384;
+int lanes_for(int64_t d) {                             // lanes of a team: eight columns each
+    const int64_t v = ceil_div(d, 8);
+    return v <= 8 ? 8 : v <= 32 ? 32 : pow2_at_least(v, 64, 1024);
+}
+struct BnPlan {
+    int tpr, nt, nblk, S, na;
+    int64_t split;
+    size_t gpart, bytes;
+};
+BnPlan grad_plan(const dnag_block_norms_args &p) {
+    BnPlan q;
+    q.tpr = lanes_for(p.dim);
+    q.nt = q.tpr <= 64 ? 256 / q.tpr : 1;
+    q.na = p.layer_norm ? 4 : 2;
+    const int64_t G = p.gate_rows, rpg = p.rows / G;
+    // two blocks of 256 lanes for every CU: fewer partial sums than a block per row, and enough rows in flight
+    const int64_t target = q.tpr <= 256 ? 1024 : q.tpr == 512 ? 512 : 256;
+    q.S = 1;
+    if (rpg >= q.nt) {
+        int64_t s = ceil_div(target, G), most = ceil_div(rpg, q.nt);
+        if (s > most) s = most;
+        q.split = ceil_div(rpg, s);
+        q.S = (int)ceil_div(rpg, q.split);
+    } else q.split = rpg;
+    const int64_t items = rpg >= q.nt ? G * q.S : ceil_div(G, q.nt);
+    q.nblk = (int)(items < target ? items : target);
+    q.gpart = align256((size_t)q.nblk * q.na * p.dim * 4);
+    q.bytes = q.gpart + (q.S > 1 ? (size_t)G * q.S * p.dim * 4 : 0);
+    return q;
+}
+int check(const dnag_block_norms_args *p) {
+    if (!p) return dnag_fail(DNAG_E_ARG, "NULL pointer");
+    if (!dtype_known(p->dtype)) return dnag_fail(DNAG_E_ARG, "unknown dtype %d", p->dtype);
+    if (p->x_dtype != p->dtype && p->x_dtype != DNAG_F32) return dnag_fail(DNAG_E_ARG, "the residual stream has dtype %d: the branch's (%d) or fp32 are built", p->x_dtype, p->dtype);
+    if (p->dim < 1 || p->dim > BN_MAX_D) return dnag_fail(DNAG_E_ARG, "dim=%lld out of range (1 .. %d)", (long long)p->dim, BN_MAX_D);
+    if (p->rows < 0 || p->rows > 0x7fffffffll) return dnag_fail(DNAG_E_ARG, "rows=%lld out of range", (long long)p->rows);
+    if (p->gate_rows < 1 || (p->rows > 0 && p->rows % p->gate_rows)) return dnag_fail(DNAG_E_ARG, "%lld rows do not divide into %lld gate rows", (long long)p->rows, (long long)p->gate_rows);
+    if (!p->layer_norm && (p->post_bias || p->pre_bias)) return dnag_fail(DNAG_E_ARG, "RMSNorm has no bias");
+    if (!p->y && !p->pre) return dnag_fail(DNAG_E_ARG, "without y there is only the norm in front: pre must be set");
+    if (!p->y && (p->gate || p->post_weight || p->post_bias)) return dnag_fail(DNAG_E_ARG, "gate and post norm need y");
+    if (!p->pre && (p->pre_weight || p->pre_bias)) return dnag_fail(DNAG_E_ARG, "pre_weight / pre_bias without pre");
+    if (p->x_stride < p->dim || (p->y && p->y_stride < p->dim)) return dnag_fail(DNAG_E_ARG, "a row stride is smaller than dim");
+    return 0;
+}
+BnArgs common_args(const dnag_block_norms_args &p) {
+    BnArgs a = {};
+    a.x = p.x; a.y = p.y; a.gate = p.gate; a.pw = p.post_weight; a.pb = p.post_bias; a.qw = p.pre_weight; a.qb = p.pre_bias;
+    a.xs = p.x_stride; a.ys = p.y_stride;
+    a.rows = p.rows; a.G = p.gate_rows; a.rpg = p.rows / p.gate_rows;
+    a.d = (int)p.dim; a.pre = p.pre; a.small32 = p.small_f32;
+    a.rs = p.residual_scale; a.eps = p.eps; a.inv_d = 1.0f / (float)p.dim;
+    return a;
+}
+template <class TX, class TY, int TPR, int NV, bool LN>
+void launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
+    if (grad) hipLaunchKernelGGL((block_norms_grad_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(TPR <= 64 ? 256 : TPR), 0, st, a);
+    else hipLaunchKernelGGL((block_norms_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(TPR <= 64 ? 256 : TPR), 0, st, a);
+}
+template <class TX, class TY, bool LN>
+void launch_width(const BnArgs &a, int tpr, bool grad, unsigned blocks, hipStream_t st) {
+    switch (tpr) {
+        case 8: launch<TX, TY, 8, 1, LN>(a, grad, blocks, st); break;
+        case 32: launch<TX, TY, 32, 1, LN>(a, grad, blocks, st); break;
+        case 64: launch<TX, TY, 64, 1, LN>(a, grad, blocks, st); break;
+        case 128: launch<TX, TY, 128, 1, LN>(a, grad, blocks, st); break;
+        case 256: launch<TX, TY, 256, 1, LN>(a, grad, blocks, st); break;
+        case 512: launch<TX, TY, 512, 1, LN>(a, grad, blocks, st); break;
+        default:
+            if (a.d <= 8192) launch<TX, TY, 1024, 1, LN>(a, grad, blocks, st);
+            else launch<TX, TY, 1024, 2, LN>(a, grad, blocks, st);
+    }
+}
+template <class TX, class TY>
+int launch_types(const dnag_block_norms_args &p, const BnArgs &a, int tpr, bool grad, unsigned blocks) {
+    hipStream_t st = (hipStream_t)p.stream;
+    if (p.layer_norm) launch_width<TX, TY, true>(a, tpr, grad, blocks, st);
+    else launch_width<TX, TY, false>(a, tpr, grad, blocks, st);
+    TOK_TRY(hipGetLastError());
+    return 0;
+}
+int launch_all(const dnag_block_norms_args &p, const BnArgs &a, int tpr, bool grad, unsigned blocks) {
+    if (p.dtype == DNAG_F32) return launch_types<float, float>(p, a, tpr, grad, blocks);
+    if (p.dtype == DNAG_BF16) return p.x_dtype == DNAG_F32 ? launch_types<float, tbf16>(p, a, tpr, grad, blocks) : launch_types<tbf16, tbf16>(p, a, tpr, grad, blocks);
+    return p.x_dtype == DNAG_F32 ? launch_types<float, tf16>(p, a, tpr, grad, blocks) : launch_types<tf16, tf16>(p, a, tpr, grad, blocks);
+}
+}  // namespace
+
+extern "C" size_t dnag_block_norms_args_bytes(void) { return sizeof(dnag_block_norms_args); }
+
+extern "C" int dnag_block_norms_forward(const dnag_block_norms_args *p) {
+    if (int rc = check(p)) return rc;
+    if (p->rows == 0) return 0;
+    if (!p->x || (p->y && !p->x_new) || (p->pre && !p->h)) return dnag_fail(DNAG_E_ARG, "NULL pointer");
+    BnArgs a = common_args(*p);
+    a.xn = p->x_new; a.h = p->h;
+    const int tpr = lanes_for(p->dim);
+    return launch_all(*p, a, tpr, false, (unsigned)ceil_div(p->rows, tpr <= 64 ? 256 / tpr : 1));
+}
+
+extern "C" size_t dnag_block_norms_grad_workspace_bytes(const dnag_block_norms_args *p) {
+    if (check(p) || p->rows == 0) return 0;
+    return grad_plan(*p).bytes;
+}
+
+extern "C" int dnag_block_norms_grad(const dnag_block_norms_args *p) {
+    if (int rc = check(p)) return rc;
+    if (p->rows == 0) return dnag_fail(DNAG_E_ARG, "no rows: the gradients of the weights are zeros, nothing is launched");
+    if (!p->x || !p->dx || (p->y && !p->dy)) return dnag_fail(DNAG_E_ARG, "NULL pointer");
+    if ((p->d_gate && !p->gate) || (p->d_post_weight && !p->post_weight) || (p->d_post_bias && !p->post_bias) || (p->d_pre_weight && !p->pre_weight) ||
+        (p->d_pre_bias && !p->pre_bias)) return dnag_fail(DNAG_E_ARG, "a gradient is asked for an input that is not there");
+    if ((p->grad_x && p->grad_x_stride < p->dim) || (p->grad_h && p->grad_h_stride < p->dim)) return dnag_fail(DNAG_E_ARG, "a row stride is smaller than dim");
+    if (p->grad_h && !p->pre) return dnag_fail(DNAG_E_ARG, "grad_h without pre");
+    const BnPlan q = grad_plan(*p);
+    if (!p->workspace || p->workspace_bytes < q.bytes) return dnag_fail(DNAG_E_WORKSPACE, "workspace has %zu bytes, %zu are needed", p->workspace_bytes, q.bytes);
+    BnArgs a = common_args(*p);
+    a.gx = p->grad_x; a.gh = p->grad_h; a.gxs = p->grad_x_stride; a.ghs = p->grad_h_stride;
+    a.dx = p->dx; a.dy = p->dy; a.dgate = p->d_gate;
+    a.S = q.S; a.split_rows = q.split;
+    const bool weights = p->d_post_weight || p->d_post_bias || p->d_pre_weight || p->d_pre_bias;
+    a.part = weights ? (float *)p->workspace : nullptr;
+    a.gpart = (float *)((char *)p->workspace + q.gpart);
+    if (int rc = launch_all(*p, a, q.tpr, true, (unsigned)q.nblk)) return rc;
+    const bool gates = p->d_gate && q.S > 1;
+    if (!weights && !gates) return 0;
+    BnJoin j = {};
+    j.part = a.part; j.gpart = a.gpart;
+    j.out[0] = p->d_pre_weight; j.out[1] = p->d_post_weight; j.out[2] = p->d_pre_bias; j.out[3] = p->d_post_bias;
+    j.dgate = p->d_gate;
+    j.na = weights ? q.na : 0; j.nblk = q.nblk; j.S = q.S; j.d = (int)p->dim; j.small32 = p->small_f32;
+    // (without weights the part's arrays are not there: the grid's second axis holds the gate rows only)
+    const dim3 grid((unsigned)ceil_div(p->dim, 64), (unsigned)(j.na + (gates ? p->gate_rows : 0)));
+    hipStream_t st = (hipStream_t)p->stream;
+    if (p->dtype == DNAG_F32) hipLaunchKernelGGL((block_norms_join_kernel<float>), grid, dim3(1024), 0, st, j);
+    else if (p->dtype == DNAG_BF16) hipLaunchKernelGGL((block_norms_join_kernel<tbf16>), grid, dim3(1024), 0, st, j);
+    else hipLaunchKernelGGL((block_norms_join_kernel<tf16>), grid, dim3(1024), 0, st, j);
+    TOK_TRY(hipGetLastError());
+    return 0;
+}

@@ -35,6 +35,15 @@ static int fail(int code, const char *fmt, ...) {
     return code;
 }
 
+// the same for the library's other translation units (dnag_token_common.h)
+__attribute__((visibility("hidden"))) int dnag_fail(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
 #define HIP_TRY(expr)                                                                                  \
     do {                                                                                               \
         hipError_t e_ = (expr);                                                                        \

@@ -29,7 +29,10 @@ def reset_seed(seed):
 def generate_archs_meta(config, sampling_fn, score_model, score_ema, meta_surrogate_model, num_samples, args=None, task=None,
                         patient_factor=20, batch_size=256):
     """Same arguments and return value (list of unique valid architecture strings) as the reference.
-    ``score_ema`` may be None when the model already holds the EMA weights."""
+    ``score_ema`` may be None when the model already holds the EMA weights.
+
+    ``args.draw_temperature`` (absent or 0: the reference's threshold) ends a round by drawing one operation per node from the
+    sampler's output at that temperature (``utils.draw_onehot``; also ``args.draw_top_p``, ``args.draw_min_p``)."""
     mask_s = utils.aug_mask(utils.nb201_adj())[0].to(config.device)                 # :118-124 (default algo 'floyed')
     if score_ema is not None:
         score_ema.copy_to(score_model.parameters())                                  # :126
@@ -42,6 +45,11 @@ def generate_archs_meta(config, sampling_fn, score_model, score_ema, meta_surrog
     while rnd < num_sampling_rounds:                                                 # :134
         rnd += 1
         sample = sampling_fn(score_model, mask_s, meta_surrogate_model, classifier_scale=c_scale, task=task)
+        draw = float(getattr(args, "draw_temperature", 0.0))
+        if draw > 0:
+            u = torch.rand(sample.shape[:-1], device=sample.device)
+            sample = utils.draw_onehot(sample, u, temperature=draw, top_p=float(getattr(args, "draw_top_p", 1.0)),
+                                       min_p=float(getattr(args, "draw_min_p", 0.0)))
         _, _, counts = AF.device_validity(sample, seen, base)
         base += sample.shape[0]
         c_scale -= args.scale_step                                                   # :145

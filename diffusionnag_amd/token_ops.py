@@ -1,0 +1,510 @@
+"""Operators of token models on the HIP library: embedding lookup, the norms between blocks, distillation from a teacher's top
+logits, and drawing tokens.
+
+They stand beside the score network's own parts: ``embed_tokens`` is the embedding of nodes whose type is known (the
+score network embeds real vectors, ``cate.py``), ``block_norms`` the seam that its encoder layers have inside the fused kernel,
+``distill_loss`` a training loss like ``losses.get_sde_loss_fn_nas``, and ``sample_tokens`` the drawing counterpart of the
+threshold ``utils.quantize`` (``utils.draw_onehot`` ends a sampling round with it).
+
+Each operator is one call on the current stream.  Tensors live on one HIP device (there is no CPU path); inputs with a
+contiguous last dimension are read in place, others are copied first; outputs are new contiguous tensors, workspaces come from torch's
+allocator and belong to the call (also under graph capture).  The first three are differentiable through ``torch.autograd``;
+``embed_tokens_grad``, ``block_norms_grad`` and ``distill_loss_and_grad`` give the same gradients without it, which is also how to
+capture a training step into a graph: a backward pass of ``torch.autograd`` that is captured while an eager graph of the
+same leaves is alive ends the process inside torch, so the differentiable calls raise there.
+Element types: float32, bfloat16, float16.  All sums and statistics are float32 or wider; results are rounded once.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_REDUCE = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
+_IDS = {torch.int32: 4, torch.int64: 8}
+
+Number = Union[int, float]
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# plumbing
+# ---------------------------------------------------------------------------------------------------------------
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} has dtype {t.dtype}; float32, bfloat16 and float16 are built")
+    return code
+
+
+class _on:
+    """The device as current for the call, if it is not already (torch.cuda.device without its cost where nothing changes)."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[..., d] as [rows, d] with a contiguous last dimension and one row stride; a copy only where the strides ask for it."""
+    d = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, d) if d else t.reshape(t.numel(), 0)
+    if t.shape[0] > 1 and t.stride(0) < d or (d > 1 and t.stride(1) != 1):
+        t = t.contiguous()
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _p(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _leaf_mark(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses to record a backward pass of leaves under graph capture while an eager graph of the same leaves is alive: their
+    gradient accumulators belong to the eager graph's stream, and running them inside the capture ends the process."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    for t in tensors:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        node = torch.autograd.graph.get_gradient_edge(t).node
+        if not capturing:
+            node.metadata["dnag_eager"] = True
+        elif node.metadata.get("dnag_eager"):
+            raise RuntimeError("an eager autograd graph of the same parameters is alive: free it before capturing, or capture the "
+                               "explicit *_grad calls of diffusionnag_amd.token_ops")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# embedding lookup
+# ---------------------------------------------------------------------------------------------------------------
+def _check_ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in _IDS:
+        raise ValueError(f"ids have dtype {ids.dtype}; int32 and int64 are built")
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def _embed(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    lib = _lib.load()
+    dev = _lib.require_device(ids, weight)
+    out = torch.empty(ids.shape + (weight.shape[1],), dtype=weight.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    w = weight.detach()
+    if w.stride(1) != 1 and w.shape[1] > 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
+        w = w.contiguous()
+    with _on(dev) as stream:
+        _lib.check(lib.dnag_embed_forward(ids.data_ptr(), _IDS[ids.dtype], ids.numel(), w.data_ptr(), _row_stride(w), w.shape[0], w.shape[1],
+                                          _dtype(weight, "weight"), scale, out.data_ptr(), stream), "dnag_embed_forward")
+    return out
+
+
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = weight.shape[0], scale, padding_idx
+        return _embed(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        num_tokens, scale, padding_idx = ctx.args
+        return None, embed_tokens_grad(grad, ids, num_tokens, scale=scale, padding_idx=padding_idx), None, None
+
+
+def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: Number = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[ids]`` ([*ids.shape, d], the type of ``weight``), rounded once.
+
+    ``ids`` outside ``0 .. len(weight) - 1`` (the -1 or -100 of a padded batch, another shard's tokens) give rows of zeros and
+    take no part in the gradient; ``padding_idx`` is looked up but takes no part in the gradient (as in torch)."""
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be [num_tokens, dim], got {tuple(weight.shape)}")
+    _dtype(weight, "weight")
+    ids = _check_ids(ids)
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {weight.shape[0] - 1}")
+    if weight.requires_grad and torch.is_grad_enabled():
+        _lib.require_device(ids, weight)
+        _leaf_mark(weight)
+        return _EmbedTokens.apply(ids, weight, float(scale), padding_idx)
+    return _embed(ids, weight, float(scale))
+
+
+def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *, scale: Number = 1.0,
+                      padding_idx: Optional[int] = None) -> torch.Tensor:
+    """Gradient of ``embed_tokens`` with respect to ``weight`` ([num_tokens, d], the type of ``grad``): the rows of ``grad``
+    summed by token in float32, in the order of the tokens' positions, the same bits every time."""
+    lib = _lib.load()
+    ids = _check_ids(ids)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
+        raise ValueError(f"grad {tuple(grad.shape)} does not match ids {tuple(ids.shape)}")
+    if num_tokens < 1 or grad.shape[-1] < 1:
+        raise ValueError(f"num_tokens={num_tokens}, dim={grad.shape[-1]}: both must be positive")
+    code = _dtype(grad, "grad")
+    dev = _lib.require_device(grad, ids)
+    g = _rows2d(grad.detach())
+    rows, d = g.shape
+    out = torch.empty(num_tokens, d, dtype=grad.dtype, device=dev)
+    nbytes = lib.dnag_embed_grad_workspace_bytes(rows, num_tokens, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as stream:
+        _lib.check(lib.dnag_embed_grad(ids.data_ptr(), _IDS[ids.dtype], rows, g.data_ptr(), max(_row_stride(g), d), num_tokens, d, code, float(scale),
+                                       -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _p(ws), nbytes, stream), "dnag_embed_grad")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# norms between blocks
+# ---------------------------------------------------------------------------------------------------------------
+class BlockNormsGrad(NamedTuple):
+    """Gradients of ``block_norms``, named like its arguments; None where the argument was not given."""
+    x: torch.Tensor
+    y: Optional[torch.Tensor]
+    gate: Optional[torch.Tensor]
+    post_weight: Optional[torch.Tensor]
+    post_bias: Optional[torch.Tensor]
+    pre_weight: Optional[torch.Tensor]
+    pre_bias: Optional[torch.Tensor]
+
+
+class _Seam:
+    """The checked arguments of one ``block_norms`` call as the library takes them."""
+
+    def __init__(self, x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype=None):
+        if norm not in ("rms", "layer"):
+            raise ValueError(f"norm={norm!r}: 'rms' and 'layer' are built")
+        if not eps >= 0:
+            raise ValueError(f"eps={eps} must not be negative")
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise ValueError(f"x must be [..., dim], got {tuple(x.shape)}")
+        if y is not None and y.shape != x.shape:
+            raise ValueError(f"y {tuple(y.shape)} does not match x {tuple(x.shape)}")
+        if y is None and (gate is not None or post_weight is not None or post_bias is not None):
+            raise ValueError("gate and the norm behind a block need its output y")
+        if y is None and not pre:
+            raise ValueError("without y there is only the norm in front of the next block: pre must be True")
+        if not pre and (pre_weight is not None or pre_bias is not None):
+            raise ValueError("pre_weight / pre_bias with pre=False")
+        if norm == "rms" and (post_bias is not None or pre_bias is not None):
+            raise ValueError("RMSNorm has no bias")
+        if dtype is not None and y is not None and dtype != y.dtype:
+            raise ValueError("dtype is the type of h at the entry (y=None); with y, h has the type of y")
+        d = x.shape[-1]
+        self.type = y.dtype if y is not None else (dtype or x.dtype)
+        if self.type not in _DTYPES:
+            raise ValueError(f"dtype {self.type}; float32, bfloat16 and float16 are built")
+        if x.dtype not in (self.type, torch.float32):
+            raise ValueError(f"x has dtype {x.dtype}; the branch's ({self.type}) or float32 are built")
+        if d > 16384:
+            raise ValueError(f"dim={d}: 1 to 16384 are built")
+        self.x, self.y = _rows2d(x.detach()), None if y is None else _rows2d(y.detach())
+        rows = self.x.shape[0]
+        self.rows, self.d, self.shape = rows, d, x.shape
+        small, f32 = {}, 0
+        for bit, names in ((2, (("post_weight", post_weight), ("post_bias", post_bias))), (4, (("pre_weight", pre_weight), ("pre_bias", pre_bias)))):
+            have = [t for _, t in names if t is not None]
+            for name, t in names:
+                if t is None:
+                    continue
+                if t.shape != (d,):
+                    raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
+                if t.dtype not in (self.type, torch.float32) or t.dtype != have[0].dtype:
+                    raise ValueError(f"{name} has dtype {t.dtype}; the branch's ({self.type}) or float32 are built, one for a norm's weight and bias")
+                small[name] = t.detach().contiguous()
+            if have and have[0].dtype == torch.float32:
+                f32 |= bit
+        self.gate_rows, self.gate = 1, None
+        if gate is not None:
+            if gate.shape[-1:] != (d,) or gate.dtype not in (self.type, torch.float32):
+                raise ValueError(f"gate must be [..., {d}] of type {self.type} or float32, got {tuple(gate.shape)} {gate.dtype}")
+            self.gate = gate.detach().contiguous()
+            self.gate_rows = gate.numel() // d
+            if self.gate_rows < 1 or rows % self.gate_rows:
+                raise ValueError(f"{rows} rows do not divide into {self.gate_rows} gate rows")
+            if gate.dtype == torch.float32:
+                f32 |= 1
+        self.dev = _lib.require_device(x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+        a = self.args = _lib.BlockNormsArgsC()
+        a.rows, a.dim, a.gate_rows = rows, d, self.gate_rows
+        a.dtype, a.x_dtype, a.layer_norm, a.pre, a.small_f32 = _DTYPES[self.type], _DTYPES[x.dtype], int(norm == "layer"), int(bool(pre)), f32
+        a.residual_scale, a.eps = float(residual_scale), float(eps)
+        a.x, a.x_stride = self.x.data_ptr(), max(_row_stride(self.x), d)
+        if self.y is not None:
+            a.y, a.y_stride = self.y.data_ptr(), max(_row_stride(self.y), d)
+        a.gate = _p(self.gate)
+        for name, t in small.items():
+            setattr(a, name, t.data_ptr())
+        self.small = small                     # keeps the tensors alive for the call
+
+    def forward(self):
+        a = self.args
+        x_new = torch.empty(self.shape, dtype=self.x.dtype, device=self.dev) if self.y is not None else None
+        h = torch.empty(self.shape, dtype=self.type, device=self.dev) if a.pre else None
+        if self.rows:
+            a.x_new, a.h = _p(x_new), _p(h)
+            with _on(self.dev) as a.stream:
+                _lib.check(_lib.load().dnag_block_norms_forward(C.byref(a)), "dnag_block_norms_forward")
+        return x_new, h
+
+    def backward(self, grad_x, grad_h, wanted) -> BlockNormsGrad:
+        a, dev = self.args, self.dev
+        if grad_x is not None:
+            if grad_x.shape != self.shape or grad_x.dtype != self.x.dtype:
+                raise ValueError(f"grad_x must be {tuple(self.shape)} of type {self.x.dtype}, got {tuple(grad_x.shape)} {grad_x.dtype}")
+            grad_x = _rows2d(grad_x.detach())
+            a.grad_x, a.grad_x_stride = grad_x.data_ptr(), max(_row_stride(grad_x), self.d)
+        if grad_h is not None:
+            if not a.pre:
+                raise ValueError("grad_h with pre=False")
+            if grad_h.shape != self.shape or grad_h.dtype != self.type:
+                raise ValueError(f"grad_h must be {tuple(self.shape)} of type {self.type}, got {tuple(grad_h.shape)} {grad_h.dtype}")
+            grad_h = _rows2d(grad_h.detach())
+            a.grad_h, a.grad_h_stride = grad_h.data_ptr(), max(_row_stride(grad_h), self.d)
+        _lib.require_device(self.x, grad_x, grad_h)
+        dx = torch.empty(self.shape, dtype=self.x.dtype, device=dev)
+        dy = torch.empty(self.shape, dtype=self.type, device=dev) if self.y is not None else None
+        new = torch.empty if self.rows else torch.zeros
+        grads = {n: new(self.d, dtype=t.dtype, device=dev) for n, t in self.small.items() if n in wanted}
+        dgate = new(self.gate.shape, dtype=self.gate.dtype, device=dev) if self.gate is not None and "gate" in wanted else None
+        if self.rows:
+            a.dx, a.dy, a.d_gate = dx.data_ptr(), _p(dy), _p(dgate)
+            for n, t in grads.items():
+                setattr(a, "d_" + n, t.data_ptr())
+            lib = _lib.load()
+            nbytes = lib.dnag_block_norms_grad_workspace_bytes(C.byref(a))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+            with _on(dev) as a.stream:
+                _lib.check(lib.dnag_block_norms_grad(C.byref(a)), "dnag_block_norms_grad")
+        return BlockNormsGrad(dx, dy, dgate, grads.get("post_weight"), grads.get("post_bias"), grads.get("pre_weight"), grads.get("pre_bias"))
+
+
+_SMALL = ("gate", "post_weight", "post_bias", "pre_weight", "pre_bias")
+
+
+class _BlockNorms(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, norm, eps, pre, dtype):
+        seam = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype)
+        ctx.save_for_backward(x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+        ctx.args = residual_scale, norm, eps, pre, dtype
+        ctx.set_materialize_grads(False)
+        x_new, h = seam.forward()
+        return tuple(t for t in (x_new, h) if t is not None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        x, y, gate, post_weight, post_bias, pre_weight, pre_bias = ctx.saved_tensors
+        residual_scale, norm, eps, pre, dtype = ctx.args
+        grad_x = grads[0] if y is not None else None
+        grad_h = grads[-1] if pre else None
+        if grad_x is None and grad_h is None:
+            return (None,) * 12
+        wanted = {n for n, need in zip(_SMALL, ctx.needs_input_grad[2:7]) if need}
+        g = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype).backward(grad_x, grad_h, wanted)
+        return tuple(g) + (None,) * 5
+
+
+def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optional[torch.Tensor] = None, residual_scale: Number = 1.0,
+                post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                pre_weight: Optional[torch.Tensor] = None, pre_bias: Optional[torch.Tensor] = None,
+                norm: str = "rms", eps: float = 1e-6, pre: bool = True, dtype: Optional[torch.dtype] = None):
+    """The seam between two blocks: ``x_new = residual_scale * x + gate * N_post(y)`` and ``h = N_pre(x_new)``; returns
+    ``(x_new, h)``.
+
+    ``x`` [..., d] is the residual stream (the branch's type, or float32 beside a 16-bit branch), ``y`` the block's output.
+    ``norm``: 'rms' (no bias) or 'layer'.  ``y=None`` is the entry of the first block: ``(x, N_pre(x))``, with ``dtype`` the type of
+    ``h`` (default: that of ``x``); ``pre=False`` the exit of the last one: ``(x_new, None)``.  ``h`` is computed from
+    the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, ...): every G-th part of the rows of ``x``, in order,
+    uses one.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
+    tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _leaf_mark(*tensors)
+        out = _BlockNorms.apply(*tensors, residual_scale, norm, eps, pre, dtype)
+        if y is None:
+            return x, out[0]
+        return out if pre else (out[0], None)
+    x_new, h = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype).forward()
+    return (x if y is None else x_new), h
+
+
+def block_norms_grad(grad_x: Optional[torch.Tensor], grad_h: Optional[torch.Tensor], x: torch.Tensor, y: Optional[torch.Tensor] = None, *,
+                     gate: Optional[torch.Tensor] = None, residual_scale: Number = 1.0, post_weight: Optional[torch.Tensor] = None,
+                     post_bias: Optional[torch.Tensor] = None, pre_weight: Optional[torch.Tensor] = None,
+                     pre_bias: Optional[torch.Tensor] = None, norm: str = "rms", eps: float = 1e-6, pre: bool = True,
+                     dtype: Optional[torch.dtype] = None) -> BlockNormsGrad:
+    """Gradients of ``block_norms`` (same arguments) for ``grad_x`` and ``grad_h``, the gradients of ``x_new`` and ``h`` (None: zero).
+    Nothing of the forward pass but its inputs is needed.  Sums over rows run in one fixed order."""
+    seam = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype)
+    return seam.backward(grad_x, grad_h, _SMALL)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# distillation
+# ---------------------------------------------------------------------------------------------------------------
+class _Distill:
+    """The checked arguments of one distillation call as the library takes them."""
+
+    def __init__(self, logits, teacher_ids, teacher_logits, temperature, row_weight, reduction):
+        if logits.dim() < 1 or logits.shape[-1] < 1:
+            raise ValueError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
+        if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() != logits.dim() or teacher_ids.shape[:-1] != logits.shape[:-1]:
+            raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} must be "
+                             f"[..., k] beside logits {tuple(logits.shape)}")
+        if not 1 <= teacher_ids.shape[-1] <= 1024:
+            raise ValueError(f"k={teacher_ids.shape[-1]} teacher entries; 1 to 1024 are built")
+        if reduction not in _REDUCE:
+            raise ValueError(f"reduction={reduction!r}: 'none', 'sum' and 'mean' are built")
+        if not 0 < temperature < float("inf"):
+            raise ValueError(f"temperature={temperature} must be positive and finite")
+        if teacher_ids.dtype not in _IDS:
+            raise ValueError(f"teacher_ids have dtype {teacher_ids.dtype}; int32 and int64 are built")
+        self.lead = logits.shape[:-1]
+        if row_weight is not None and (row_weight.shape != self.lead or row_weight.dtype != torch.float32):
+            raise ValueError(f"row_weight must be {tuple(self.lead)} float32, got {tuple(row_weight.shape)} {row_weight.dtype}")
+        self.dev = _lib.require_device(logits, teacher_ids, teacher_logits, row_weight)
+        self.logits = _rows2d(logits.detach())
+        self.kept = (teacher_ids.contiguous(), teacher_logits.detach().contiguous(), None if row_weight is None else row_weight.detach().contiguous())
+        self.rows, self.V = self.logits.shape
+        self.reduction = reduction
+        a = self.args = _lib.DistillArgsC()
+        a.rows, a.vocab, a.logits_stride = self.rows, self.V, max(_row_stride(self.logits), self.V)
+        a.k, a.dtype, a.teacher_dtype = teacher_ids.shape[-1], _dtype(logits, "logits"), _dtype(teacher_logits, "teacher_logits")
+        a.ids_bytes, a.reduction, a.temperature = _IDS[teacher_ids.dtype], _REDUCE[reduction], float(temperature)
+        a.logits, a.teacher_ids, a.teacher_logits, a.row_weight = self.logits.data_ptr(), _p(self.kept[0]), _p(self.kept[1]), _p(self.kept[2])
+
+    def _call(self, fn: str) -> None:
+        a, lib = self.args, _lib.load()
+        nbytes = lib.dnag_distill_workspace_bytes(C.byref(a))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        with _on(self.dev) as a.stream:
+            _lib.check(getattr(lib, fn)(C.byref(a)), fn)
+
+    def loss(self, stats: bool = False, grad: bool = False):
+        a = self.args
+        none = self.reduction == "none"
+        loss = (torch.empty if self.rows else torch.zeros)(self.lead if none else (), dtype=torch.float32, device=self.dev)
+        st = torch.empty(self.rows, 2, dtype=torch.float32, device=self.dev) if stats else None
+        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.dev) if grad else None
+        if self.rows:
+            a.loss, a.stats, a.grad = loss.data_ptr(), _p(st), _p(g)
+            self._call("dnag_distill_loss_grad" if grad else "dnag_distill_loss")
+        return loss, st, g
+
+    def backward(self, stats, grad_out):
+        a = self.args
+        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.dev)
+        if self.rows:
+            up = grad_out.detach().to(torch.float32).contiguous()
+            a.stats, a.grad_out, a.grad = stats.data_ptr(), up.data_ptr(), g.data_ptr()
+            self._call("dnag_distill_backward")
+        return g
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, temperature, row_weight, reduction):
+        loss, stats, _ = _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss(stats=True)
+        ctx.save_for_backward(logits, teacher_ids, teacher_logits, row_weight, stats)
+        ctx.args = temperature, reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        logits, teacher_ids, teacher_logits, row_weight, stats = ctx.saved_tensors
+        temperature, reduction = ctx.args
+        return (_Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).backward(stats, grad_out),) + (None,) * 5
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *, temperature: Number = 1.0,
+                 row_weight: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+    """``tau^2 KL(p || q)`` for each row of ``logits`` [..., vocab]: ``q`` the student's distribution at temperature ``tau`` over the
+    whole vocabulary, ``p`` the teacher's over its k listed tokens, ``softmax(teacher_logits / tau)``.
+
+    ``teacher_ids`` [..., k] outside ``0 .. vocab - 1`` are no entries (a row shorter than k is filled with -1); repeated ids add up.
+    ``row_weight`` [...] float32: rows whose weight is not positive (padding) count nothing and their logits do not
+    matter, NaN included.  A row without entries counts 0.  ``reduction``: 'mean' over the positive weights (over all rows
+    without weights; 0 where there are none), 'sum', or 'none' (weighted loss of each row).  float32.  No gradient reaches the
+    teacher or the weights: they must not require one."""
+    if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
+        raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")
+    if logits.requires_grad and torch.is_grad_enabled():
+        _leaf_mark(logits)
+        return _DistillLoss.apply(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction)
+    return _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss()[0]
+
+
+def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *, temperature: Number = 1.0,
+                          row_weight: Optional[torch.Tensor] = None, reduction: str = "mean"):
+    """``distill_loss`` and its gradient with respect to ``logits`` (for an upstream gradient of 1) in one pass over the logits: two
+    thirds of the memory traffic of the loss followed by its backward pass.  Returns ``(loss, grad)``."""
+    loss, _, grad = _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss(grad=True)
+    return loss, grad
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# drawing
+# ---------------------------------------------------------------------------------------------------------------
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[Number, torch.Tensor] = 1.0,
+                  top_k: Union[int, torch.Tensor] = 0, top_p: Union[Number, torch.Tensor] = 1.0,
+                  min_p: Union[Number, torch.Tensor] = 0.0) -> torch.Tensor:
+    """One token per row of ``logits`` [..., vocab] (int64 [...]), drawn with the uniform numbers ``u`` [...] (float32, [0, 1)).
+
+    Order of the filters: ``temperature`` (<= 0: the largest logit), ``top_k`` (<= 0: off), ``top_p`` on what top-k left (>= 1: off,
+    at least one token stays), ``min_p`` relative to the largest probability (the largest stays).  Equal logits rank by
+    index.  The token is the first one, in index order, whose running sum of kept probability exceeds ``u`` times the total.
+    NaN and -inf are never drawn; a row of nothing else gives -1.  Each setting is a number, or a tensor with a value per
+    row (float32; int32 for ``top_k``).  The same inputs give the same tokens, whatever else runs.  vocab <= 2^20."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
+    lead = logits.shape[:-1]
+    if u.shape != lead or u.dtype != torch.float32:
+        raise ValueError(f"u must be {tuple(lead)} float32, got {tuple(u.shape)} {u.dtype}")
+    a = _lib.SampleArgsC()
+    a.dtype = _dtype(logits, "logits")
+    kept = []
+    for name, value, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                              ("min_p", min_p, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            if value.shape != lead or value.dtype != kind:
+                raise ValueError(f"{name} must be a number or {tuple(lead)} {kind}, got {tuple(value.shape)} {value.dtype}")
+            value = value.contiguous()
+            kept.append(value)
+            setattr(a, name + "_rows", value.data_ptr())
+        else:
+            if value != value or value in (float("inf"), float("-inf")):
+                raise ValueError(f"{name}={value} must be finite")
+            setattr(a, name, max(-1, min(int(value), 0x7fffffff)) if name == "top_k" else float(value))
+    dev = _lib.require_device(logits, u, *kept)
+    lg = _rows2d(logits.detach())
+    uc = u.contiguous()
+    out = torch.empty(lead, dtype=torch.int64, device=dev)
+    a.rows, a.vocab, a.logits_stride = lg.shape[0], lg.shape[1], max(_row_stride(lg), lg.shape[1])
+    if a.rows:
+        a.logits, a.u, a.out = lg.data_ptr(), uc.data_ptr(), out.data_ptr()
+        with _on(dev) as a.stream:
+            _lib.check(_lib.load().dnag_sample_tokens(C.byref(a)), "dnag_sample_tokens")
+    return out

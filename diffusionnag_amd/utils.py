@@ -122,6 +122,16 @@ def quantize(x):
     return [host[i] for i in range(host.shape[0])]
 
 
+def draw_onehot(x, u, **settings):
+    """The drawing counterpart of ``quantize``: reads every row of the sampler's output ``x`` [..., V] as logits over the V node
+    types, draws one type per row with the uniform numbers ``u`` [...] (``token_ops.sample_tokens``, which takes the
+    ``settings``: temperature, top_k, top_p, min_p) and returns one-hot rows on the device (float32, the shape of ``x``), ready for
+    ``arch_functions.device_validity``.  A row with nothing to draw stays zero."""
+    from .token_ops import sample_tokens
+    t = sample_tokens(x, u, **settings)
+    return (t.unsqueeze(-1) == torch.arange(x.shape[-1], device=x.device)).to(torch.float32)
+
+
 # ---------------------------------------------------------------------------------------------------
 # Checkpoints (reference ``utils.py:84-121``; layout in SURVEY.md Appendix C)
 # ---------------------------------------------------------------------------------------------------

@@ -386,6 +386,110 @@ int dnag_ofa_validity(const float *x, int batch, int32_t *status, int8_t *types,
  * q[i] = x[i] >= 0.5 ? 1 : 0, n elements, device pointers. */
 int dnag_quantize(const float *x, float *q, size_t n, void *stream);
 
+/* ---- operators of token models ---------------------------------------------------------------------
+ * What stands around the blocks of a network over tokens (the node types of an architecture, or any vocabulary): the
+ * embedding lookup, the norms between blocks, distillation from a teacher's top logits, drawing tokens.  No counterpart in
+ * the reference, whose nodes enter as real vectors and leave through a threshold.  diffusionnag_amd/token_ops.py is the
+ * Python face.  Element types: */
+#define DNAG_F32  0
+#define DNAG_BF16 1
+#define DNAG_F16  2
+
+/* Embedding lookup: out[t] = scale * weight[ids[t]], rounded once; an id outside 0 .. num_tokens - 1 gives a row of zeros.
+ * ids: rows int32 (ids_bytes 4) or int64 (8); weight: num_tokens rows of `dim` elements, weight_stride elements apart; out:
+ * [rows][dim].  Rows may start at any element (no alignment beyond the element's own). */
+int dnag_embed_forward(const void *ids, int ids_bytes, int64_t rows, const void *weight, int64_t weight_stride,
+                       int64_t num_tokens, int64_t dim, int dtype, float scale, void *out, void *stream);
+/* Its gradient: out[v] = scale * sum over t with ids[t] = v of grad[t], in fp32 and in one fixed order (the same bits every
+ * time), rounded once to `dtype`.  Every row of out [num_tokens][dim] is written: zeros for tokens that do not occur and for
+ * padding_idx (negative: none).  The workspace may be reused as soon as the stream has passed the call. */
+size_t dnag_embed_grad_workspace_bytes(int64_t rows, int64_t num_tokens, int64_t dim);
+int dnag_embed_grad(const void *ids, int ids_bytes, int64_t rows, const void *grad, int64_t grad_stride, int64_t num_tokens,
+                    int64_t dim, int dtype, float scale, int64_t padding_idx, void *out, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* The seam between two blocks: x_new = residual_scale * x + gate * N_post(y), h = N_pre(x_new).  N: RMSNorm, or LayerNorm
+ * (layer_norm = 1, the only one with biases), each over `dim` elements with fp32 statistics; weight / bias NULL: 1 / 0.
+ * y NULL (entry of the first block): h = N_pre(x), x_new is not written.  pre = 0 (exit of the last block): no h.
+ * gate: [gate_rows][dim], row r of x uses gate row r / (rows / gate_rows); NULL: 1.  x, x_new, grad_x, dx are of type
+ * x_dtype (dtype or DNAG_F32), everything else of type dtype, except the arrays named in small_f32 (bit 0 gate, bit 1 post_weight and
+ * post_bias, bit 2 pre_weight and pre_bias: fp32, with their gradients).  Outputs are contiguous, inputs have row strides.
+ * dnag_block_norms_grad reads x, y and the weights again (x_new and h are not needed) and grad_x, grad_h (gradients of x_new
+ * and h; NULL: zero); it writes dx and dy whole, and those of d_gate, d_post_weight, d_post_bias, d_pre_weight, d_pre_bias that
+ * are not NULL, in one fixed order of summation.  1 <= dim <= 16384. */
+typedef struct dnag_block_norms_args {
+    int64_t rows, dim, gate_rows;
+    int32_t dtype, x_dtype, layer_norm, pre, small_f32;
+    float residual_scale, eps;
+    const void *x, *y, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+    int64_t x_stride, y_stride;
+    void *x_new, *h;                                        /* forward */
+    const void *grad_x, *grad_h;                            /* backward */
+    int64_t grad_x_stride, grad_h_stride;
+    void *dx, *dy, *d_gate, *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
+    void *workspace;                                        /* backward only: dnag_block_norms_grad_workspace_bytes */
+    size_t workspace_bytes;
+    void *stream;
+} dnag_block_norms_args;
+size_t dnag_block_norms_args_bytes(void);
+size_t dnag_block_norms_grad_workspace_bytes(const dnag_block_norms_args *args);
+int dnag_block_norms_forward(const dnag_block_norms_args *args);
+int dnag_block_norms_grad(const dnag_block_norms_args *args);
+
+/* Distillation: KL divergence between the teacher's distribution over its `k` listed tokens and the student's over the whole
+ * vocabulary, both at `temperature` (tau), times tau^2:  loss_t = w_t tau^2 sum_k p_k (log p_k - log q_{id_k}).
+ * logits [rows][vocab] (row stride logits_stride) of type dtype; teacher_ids [rows][k] (ids_bytes 4 or 8; an id outside
+ * 0 .. vocab - 1 is no entry, ids may repeat), teacher_logits [rows][k] of type teacher_dtype; row_weight fp32 [rows] or NULL.
+ * A row without entries, or whose weight is not positive, counts 0 and its logits do not matter.
+ * reduction: none: loss [rows]; sum: loss [1]; mean: loss [1] = sum / sum of the positive weights (0 if there are none), or / rows.
+ * dnag_distill_loss: loss, and stats fp32 [rows][2] (may be NULL) for dnag_distill_backward.
+ * dnag_distill_loss_grad: loss and grad [rows][vocab] (type dtype, contiguous) = d loss / d logits in one pass over the logits.
+ * dnag_distill_backward: grad = d loss / d logits times grad_out (fp32 [1], or [rows] with reduction none).
+ * 1 <= k <= 1024. */
+#define DNAG_REDUCE_NONE 0
+#define DNAG_REDUCE_SUM  1
+#define DNAG_REDUCE_MEAN 2
+typedef struct dnag_distill_args {
+    int64_t rows, vocab, logits_stride;
+    int32_t k, dtype, teacher_dtype, ids_bytes, reduction;
+    float temperature;
+    const void *logits, *teacher_ids, *teacher_logits;
+    const float *row_weight;
+    float *loss, *stats;
+    const float *grad_out;
+    void *grad;
+    void *workspace;                                        /* dnag_distill_workspace_bytes */
+    size_t workspace_bytes;
+    void *stream;
+} dnag_distill_args;
+size_t dnag_distill_args_bytes(void);
+size_t dnag_distill_workspace_bytes(const dnag_distill_args *args);
+int dnag_distill_loss(const dnag_distill_args *args);
+int dnag_distill_loss_grad(const dnag_distill_args *args);
+int dnag_distill_backward(const dnag_distill_args *args);
+
+/* Drawing one token per row.  With e_i = exp((l_i - max l) / temperature): top_k keeps the k largest logits (<= 0: all), top_p of
+ * those the shortest run of largest ones that holds top_p of their sum (>= 1: all; one at least), min_p of those the ones
+ * with e_i >= min_p (the largest always); equal logits rank by index.  The token is the first, in index order, whose running sum
+ * of kept e exceeds u times their total; u in [0, 1) is the caller's.  temperature <= 0: the largest logit (lowest index).
+ * NaN and -inf are never drawn; a row of nothing else gives -1.  Weights are whole numbers of 2^-40 of the largest: sums are
+ * exact and the token does not depend on the order of summation.
+ * *_rows: a value per row (device, fp32 / int32), or NULL: the scalar for all rows.  out int64 [rows].  vocab <= 2^20. */
+typedef struct dnag_sample_args {
+    int64_t rows, vocab, logits_stride;
+    int32_t dtype, top_k;
+    double temperature, top_p, min_p;
+    const void *logits;
+    const float *u;
+    const float *temperature_rows;
+    const int32_t *top_k_rows;
+    const float *top_p_rows, *min_p_rows;
+    int64_t *out;
+    void *stream;
+} dnag_sample_args;
+size_t dnag_sample_args_bytes(void);
+int dnag_sample_tokens(const dnag_sample_args *args);
+
 /* ---- kernel timing for bench.py ----------------------------------------------------------------
  * While enabled, every `every`-th launch of the head GEMM (the dominant kernel) is bracketed by a
  * pair of HIP events on the launch stream.  dnag_timing_read() synchronises those events and

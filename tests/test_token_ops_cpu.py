@@ -1,0 +1,212 @@
+"""Token operators without a GPU: the oracle against differences, the refusals of the Python face and of the C entries (which
+check before they touch the device)."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from diffusionnag_amd import _lib, token_ops as ops
+from tests import token_reference as R
+
+
+def difference(f, x, v, eps=1e-5):
+    """Central difference of f along v, float64."""
+    return float((f(x + eps * v) - f(x - eps * v)) / (2 * eps))
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_block_norms_formula_against_differences(kind):
+    g = torch.Generator().manual_seed(3)
+    t = {n: torch.randn(s, generator=g, dtype=torch.float64) for n, s in
+         dict(x=(6, 5), y=(6, 5), gate=(3, 5), post_weight=(5,), pre_weight=(5,)).items()}
+    if kind == "layer":
+        t["post_bias"], t["pre_bias"] = torch.randn(5, generator=g).double(), torch.randn(5, generator=g).double()
+    cx, ch = torch.randn(6, 5, generator=g).double(), torch.randn(6, 5, generator=g).double()
+
+    def f(name, v):
+        xn, h = R.block_norms({**t, name: v}, 0.7, kind, 1e-6, True)
+        return (xn * cx).sum() + (h * ch).sum()
+    for name in t:
+        x = t[name].clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(f(name, x), x)
+        v = torch.randn(x.shape, generator=g).double()
+        want = float((grad * v).sum())
+        assert abs(difference(lambda z: f(name, z), t[name], v) - want) <= 1e-7 * max(1.0, abs(want))
+
+
+def test_distill_formula_against_differences():
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(4, 9, generator=g).double()
+    ids = torch.tensor([[1, 3, 1], [8, -1, 9], [-1, -1, 12], [0, 2, 4]])
+    tl = torch.randn(4, 3, generator=g).double()
+    w = torch.tensor([0.5, 2.0, 1.0, 0.0])
+    _, grad = R.distill(x, ids, tl, 1.7, w, "mean")
+    v = torch.randn(4, 9, generator=g).double()
+    want = float((grad * v).sum())
+    assert abs(difference(lambda z: R.distill(z, ids, tl, 1.7, w, "mean")[0], x, v) - want) <= 1e-8
+    assert not grad[2:].any()
+
+
+def test_sample_reference_knows_the_easy_cases():
+    x = [0.0, 2.0, 2.0, 1.0]
+    assert R.sample_row(x, 0.9, 0.0, 0, 1.0, 0.0) == 1                     # greedy, ties to the lowest index
+    assert R.sample_row(x, 0.99, 1.0, 1, 1.0, 0.0) == 1
+    assert R.sample_row(x, 0.99, 1.0, 2, 1.0, 0.0) == 2
+    assert R.sample_row([0.0] * 4, 0.6, 1.0, 0, 0.5, 0.0) == 1             # two of four equal ones hold half
+    assert R.sample_row([-np.inf, np.nan], 0.5, 1.0, 0, 1.0, 0.0) == -1
+    assert R.sample_row(x, 0.0, 1.0, 0, 1.0, 0.9) == 1 and R.sample_row(x, 0.99, 1.0, 0, 1.0, 0.9) == 2
+
+
+F32 = torch.float32
+
+
+def test_cpu_tensors_are_refused():
+    ids, w = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8)
+    for call in (lambda: ops.embed_tokens(ids, w), lambda: ops.embed_tokens_grad(torch.zeros(3, 8), ids, 4),
+                 lambda: ops.embed_tokens(ids, w.requires_grad_(True)),
+                 lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8)), lambda: ops.block_norms_grad(None, None, torch.zeros(2, 8)),
+                 lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)),
+                 lambda: ops.distill_loss_and_grad(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)),
+                 lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.embed_tokens(torch.zeros(3), torch.zeros(4, 8)),                                        # ids of no integer type
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int16), torch.zeros(4, 8)),
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int64), torch.zeros(4)),
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int64), torch.zeros(0, 8)),
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8, dtype=torch.float64)),
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), padding_idx=4),
+    lambda: ops.embed_tokens(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), padding_idx=-1),
+    lambda: ops.embed_tokens_grad(torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64), 4),
+    lambda: ops.embed_tokens_grad(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 0),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 9)),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), norm="batch"),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), eps=-1.0),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), eps=float("nan")),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), pre_bias=torch.zeros(8)),             # RMSNorm has no bias
+    lambda: ops.block_norms(torch.zeros(2, 8), gate=torch.zeros(8)),                                     # a gate without y
+    lambda: ops.block_norms(torch.zeros(2, 8), pre=False),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), pre=False, pre_weight=torch.zeros(8)),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), post_weight=torch.zeros(7)),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), post_weight=torch.zeros(8).half()),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), gate=torch.zeros(3, 8)),               # 2 rows, 3 gates
+    lambda: ops.block_norms(torch.zeros(2, 8).bfloat16(), torch.zeros(2, 8)),                            # 16-bit stream, 32-bit branch
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), dtype=torch.bfloat16),
+    lambda: ops.block_norms(torch.zeros(1, 16385), torch.zeros(1, 16385)),
+    lambda: ops.block_norms(torch.zeros(2, 0), torch.zeros(2, 0)),
+    lambda: ops.block_norms(torch.zeros(2, 8), torch.zeros(2, 8), norm="layer", pre_weight=torch.zeros(8), pre_bias=torch.zeros(8).half()),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 4)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(3, 3, dtype=torch.int64), torch.zeros(3, 3)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 0, dtype=torch.int64), torch.zeros(2, 0)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 1025, dtype=torch.int64), torch.zeros(2, 1025)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3), torch.zeros(2, 3)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=0.0),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=float("inf")),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), reduction="batchmean"),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), row_weight=torch.zeros(3)),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), row_weight=torch.zeros(2).half()),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3, requires_grad=True)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(3)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2).double()),
+    lambda: ops.sample_tokens(torch.zeros(2, 0), torch.zeros(2)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8).double(), torch.zeros(2)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2), temperature=torch.ones(3)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2), top_k=torch.ones(2)),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2), top_p=float("nan")),
+    lambda: ops.sample_tokens(torch.zeros(2, 8), torch.zeros(2), temperature=float("inf")),
+])
+def test_bad_arguments_are_refused(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def refused(rc, words):
+    assert rc == -1 or rc == -2, rc
+    assert words in _lib.load().dnag_last_error().decode()
+
+
+def test_c_entries_check_before_they_launch():
+    """Addresses that are not NULL stand for device memory; every call below is refused on the host."""
+    lib, P = _lib.load(), 4096
+    e = lib.dnag_embed_forward
+    refused(e(P, 8, 1, P, 8, 4, 8, 7, 1.0, P, None), "dtype")
+    refused(e(P, 2, 1, P, 8, 4, 8, 0, 1.0, P, None), "ids of 2 bytes")
+    refused(e(P, 8, -1, P, 8, 4, 8, 0, 1.0, P, None), "rows")
+    refused(e(P, 8, 1, P, 7, 4, 8, 0, 1.0, P, None), "stride")
+    refused(e(P, 8, 1, P, 8, 0, 8, 0, 1.0, P, None), "num_tokens")
+    refused(e(P, 8, 1, P, 8, 4, 0, 0, 1.0, P, None), "dim")
+    refused(e(None, 8, 1, P, 8, 4, 8, 0, 1.0, P, None), "NULL")
+    assert e(None, 8, 0, None, 8, 4, 8, 0, 1.0, None, None) == 0                      # no rows: nothing to do
+    need = lib.dnag_embed_grad_workspace_bytes(1000, 500, 64)
+    assert need > 0
+    refused(lib.dnag_embed_grad(P, 8, 1000, P, 64, 500, 64, 0, 1.0, -1, P, P, need - 1, None), "workspace")
+    refused(lib.dnag_embed_grad(P, 8, 1000, P, 64, 500, 64, 0, 1.0, -1, None, P, need, None), "NULL")
+    assert lib.dnag_embed_grad_workspace_bytes(-1, 500, 64) == 0
+
+    def norms(**kw):
+        a = _lib.BlockNormsArgsC()
+        base = dict(rows=4, dim=8, gate_rows=1, dtype=1, x_dtype=1, pre=1, x=P, y=P, x_stride=8, y_stride=8, x_new=P, h=P, eps=1e-6,
+                    grad_x=P, grad_h=P, grad_x_stride=8, grad_h_stride=8, dx=P, dy=P)
+        for k, v in {**base, **kw}.items():
+            setattr(a, k, v)
+        return a
+    for kw, words in ((dict(dtype=9), "dtype"), (dict(x_dtype=2), "residual"), (dict(dim=16385), "dim"), (dict(dim=0), "dim"), (dict(gate_rows=3), "gate rows"),
+                      (dict(post_bias=P), "no bias"), (dict(y=None, pre=0), "pre must"), (dict(y=None, gate=P), "need y"),
+                      (dict(pre=0, pre_weight=P), "without pre"), (dict(x_stride=7), "stride"), (dict(x=None), "NULL"), (dict(h=None), "NULL")):
+        refused(lib.dnag_block_norms_forward(C.byref(norms(**kw))), words)
+    assert lib.dnag_block_norms_forward(C.byref(norms(rows=0))) == 0
+    a = norms(pre_weight=P, d_pre_weight=P, workspace=P)
+    need = lib.dnag_block_norms_grad_workspace_bytes(C.byref(a))
+    a.workspace_bytes = need - 1
+    refused(lib.dnag_block_norms_grad(C.byref(a)), "workspace")
+    refused(lib.dnag_block_norms_grad(C.byref(norms(d_gate=P, workspace=P, workspace_bytes=1 << 40))), "not there")
+    refused(lib.dnag_block_norms_grad(C.byref(norms(pre=0, workspace=P, workspace_bytes=1 << 40))), "grad_h without pre")
+    refused(lib.dnag_block_norms_grad(C.byref(norms(rows=0))), "no rows")
+    refused(lib.dnag_block_norms_forward(None), "NULL")
+
+    def distill(**kw):
+        a = _lib.DistillArgsC()
+        base = dict(rows=4, vocab=8, logits_stride=8, k=3, ids_bytes=8, reduction=2, temperature=1.0, logits=P, teacher_ids=P, teacher_logits=P,
+                    loss=P, stats=P, grad_out=P, grad=P, workspace=P, workspace_bytes=1 << 20)
+        for k, v in {**base, **kw}.items():
+            setattr(a, k, v)
+        return a
+    for kw, words in ((dict(dtype=3), "dtype"), (dict(teacher_dtype=-1), "dtype"), (dict(ids_bytes=1), "ids of 1"), (dict(vocab=0), "vocab"), (dict(k=0), "k=0"),
+                      (dict(k=1025), "k=1025"), (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+                      (dict(logits_stride=7), "stride"), (dict(reduction=3), "reduction"), (dict(loss=None), "NULL"), (dict(workspace_bytes=0), "workspace"),
+                      (dict(rows=0), "no rows")):
+        refused(lib.dnag_distill_loss(C.byref(distill(**kw))), words)
+        refused(lib.dnag_distill_loss_grad(C.byref(distill(**kw))), words)
+    refused(lib.dnag_distill_loss_grad(C.byref(distill(grad=None))), "NULL")
+    refused(lib.dnag_distill_backward(C.byref(distill(stats=None))), "NULL")
+    refused(lib.dnag_distill_backward(C.byref(distill(grad_out=None))), "NULL")
+
+    def sample(**kw):
+        a = _lib.SampleArgsC()
+        base = dict(rows=4, vocab=8, logits_stride=8, temperature=1.0, top_p=1.0, logits=P, u=P, out=P)
+        for k, v in {**base, **kw}.items():
+            setattr(a, k, v)
+        return a
+    for kw, words in ((dict(dtype=3), "dtype"), (dict(rows=-1), "rows"), (dict(vocab=(1 << 20) + 1), "vocab"), (dict(vocab=0), "vocab"),
+                      (dict(logits_stride=7), "stride"), (dict(u=None), "NULL"), (dict(out=None), "NULL")):
+        refused(lib.dnag_sample_tokens(C.byref(sample(**kw))), words)
+    assert lib.dnag_sample_tokens(C.byref(sample(rows=0))) == 0
+
+
+def test_eager_graph_of_the_same_leaf_is_noticed(monkeypatch):
+    """_leaf_mark: a leaf whose gradient accumulator lives on from an eager graph is refused under capture, a fresh one is not."""
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    w = torch.zeros(3, requires_grad=True)
+    alive = (w * 2).sum()
+    ops._leaf_mark(w, None, torch.zeros(3))
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        ops._leaf_mark(w)
+    del alive
+    ops._leaf_mark(w)
