@@ -7,19 +7,28 @@
 // T <= 0: the largest logit's lowest index.  NaN and -inf are never drawn; a row of nothing else gives -1.
 //
 // Whole-number weights make every sum independent of its order (LDS atomics among them) and every comparison exact: the
-// token is a function of the row, whichever threads it falls to.  exp is fp64 (an fp32 one moves the border between two
-// tokens by 1e-7, which over a flat row of 10^5 tokens changes one draw in a few hundred); 2^-40 is below what a uniform
-// fp32 number resolves.  A cut (top-k, top-p) is found by histograms: 2048 equal steps of (max - l) / T, then, inside the step where the
-// sum passes its goal, eleven, eleven and ten bits of the logit's ordered bit pattern, then the index among equal logits.
-// One workgroup per row, the row read again (out of the caches) by each pass; rows of at most 64 logits take a team of
-// lanes each and rank by comparing all pairs.
+// token is a function of the row, whichever threads it falls to.  exp is fp64 arithmetic (an fp32 one moves the border between
+// two tokens by 1e-7, which over a flat row of 10^5 tokens changes one draw in a few hundred): 2^y by a polynomial that is
+// 2^-45.9 off at most, below the weights' step.  2^-40 is below what a uniform fp32 number resolves.
+//
+// One workgroup per row, which reads the row again (out of the caches) for each of its passes; bound by the instructions per
+// logit, not by HBM, so the passes are few and the exact work falls on few logits:
+//   top-k of at most as many as there are lanes: the k-th largest of the lanes' own maxima is no larger than the k-th largest
+//     logit, so the logits from there on (little more than k) hold all candidates: they are sorted in LDS and everything else --
+//     top-p, min-p, the draw -- happens on that list.
+//   otherwise a cut (top-k, top-p) is found by a histogram over 2048 equal steps of (max - l) / T; the logits in the step where
+//     the sum passes its goal are sorted (or, where they are more than the list holds, divided by eleven, eleven and ten bits of
+//     their ordered bit pattern and then by index).  The draw sums pieces of 512 logits, then looks into one piece.
+// Rows of at most 64 logits take a team of lanes each and rank by comparing all pairs.
 #include "dnag_token_common.h"
+#include <float.h>
 #include <math.h>
 
 #define SMP_BINS 2048
 #define SMP_RANGE 28.0f          // exp(-28) < 2^-40: weights beyond are 0
-#define SMP_ONE 1099511627776.0  // 2^40
+#define SMP_BITS 40
 #define SMP_MAX_V (1 << 20)      // sums stay below 2^60
+#define SMP_LIST 2048            // logits that are sorted in LDS
 
 typedef unsigned long long u64;
 
@@ -34,15 +43,15 @@ struct SampleArgs {
     int top_k1;
     int64_t *out;
 };
-struct RowSet { double it, p, minp; int k; bool greedy; };
+struct RowSet { double c, p, minw; int k; bool greedy; };      // c = log2(e) / T; minw = min_p 2^40
 __device__ __forceinline__ RowSet row_set(const SampleArgs &a, int64_t row) {
     RowSet s;
     const double t = a.temperature ? (double)a.temperature[row] : a.temperature1;
     s.greedy = !(t > 0.0);
-    s.it = 1.0 / t;
+    s.c = 1.4426950408889634074 / t;
     s.p = a.top_p ? (double)a.top_p[row] : a.top_p1;
-    s.minp = a.min_p ? (double)a.min_p[row] : a.min_p1;
-    if (s.minp != s.minp) s.minp = 0.0;
+    const double q = a.min_p ? (double)a.min_p[row] : a.min_p1;
+    s.minw = q == q ? q * 1099511627776.0 : 0.0;
     s.k = a.top_k ? a.top_k[row] : a.top_k1;
     return s;
 }
@@ -53,8 +62,28 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x);
     return b ^ (b & 0x80000000u ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ double raw_weight(float x, float m, double it) { return x == m ? 1.0 : exp(((double)x - (double)m) * it); }
-__device__ __forceinline__ u64 whole_weight(double e) { return (u64)rint(e * SMP_ONE); }
+// 2^40 exp((x - m) / T) before it is rounded, c = log2(e) / T; NaN and -inf give 2^-24 of a step.  Conversions and ldexp are slow
+// beside additions in fp64, so the whole part of y is rounded off by adding 1.5 2^52 (it lands in the low bits) and added to
+// the exponent as an integer.
+__device__ __forceinline__ double raw_weight(float x, double m, double c) {
+    const double y = fmax(((double)x - m) * c, -64.0);
+    const double t = y + 6755399441055744.0, f = y - (t - 6755399441055744.0);               // f in [-1/2, 1/2]
+    // 2^f: least relative error with p(0) = 1, fitted at 4000 points; 1.5e-14 off
+    double p = 1.0148340400913933e-07;
+    p = fma(p, f, 1.3258335536991744e-06);
+    p = fma(p, f, 1.525299001687859e-05);
+    p = fma(p, f, 0.00015403440883783207);
+    p = fma(p, f, 0.0013333557625467886);
+    p = fma(p, f, 0.009618129181164985);
+    p = fma(p, f, 0.05550410866841576);
+    p = fma(p, f, 0.24022650695722814);
+    p = fma(p, f, 0.6931471805598851);
+    p = fma(p, f, 1.0);
+    return __hiloint2double(__double2hiint(p) + ((__double2loint(t) + SMP_BITS) << 20), __double2loint(p));
+}
+__device__ __forceinline__ u64 whole_weight(double v) {        // v in [0, 2^41): rounded by the addition's own rounding
+    return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull;
+}
 __device__ __forceinline__ u64 goal_of(double p, u64 total) {          // smallest whole number >= p total, 1 at least
     const double r = ceil(p * (double)total);
     return r >= 1.0 ? (r < (double)total ? (u64)r : total) : 1;
@@ -85,7 +114,7 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const SampleArgs a, i
         }
         int pick = rank == 0 ? lane : G;               // the largest logit's lowest index
         if (!s.greedy) {
-            const double e = live ? raw_weight(x, m, s.it) : 0.0;
+            const double e = !live ? 0.0 : m == INFINITY ? (x == m ? 1099511627776.0 : 0.0) : raw_weight(x, (double)m, s.c);
             const u64 w = whole_weight(e);
             bool kept = live && (s.k <= 0 || rank < s.k);
             if (s.p < 1.0) {
@@ -100,7 +129,7 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const SampleArgs a, i
                 }
                 kept = kept && before < goal_of(s.p, total);
             }
-            kept = kept && (e >= s.minp || rank == 0);
+            kept = kept && (e >= s.minw || rank == 0);
             u64 sum = kept ? w : 0;
             for (int o = 1; o < G; o <<= 1) { const u64 b = __shfl_up(sum, o, 64); if (lane >= o) sum += b; }
             const u64 total = __shfl(sum, (threadIdx.x & 63) | (G - 1), 64);
@@ -113,68 +142,213 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const SampleArgs a, i
 }
 
 // ---- one workgroup per row -----------------------------------------------------------------------------------------------
-struct Cut {                       // kept: in an earlier step, or in this one with a larger key, or an equal key and index <= at
-    int step;
-    uint32_t key;
-    int at;
-};
+struct Cut { float x; int at; };   // kept: larger logits, and equal ones up to index `at`
+
 template <class T, int NTHR>
 __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     constexpr int NW = NTHR / 64, PER = SMP_BINS / NTHR;
     extern __shared__ u64 piece[];                     // sums of 512 logits each, for the draw
-    __shared__ u64 hist[SMP_BINS];
+    __shared__ u64 hist[SMP_BINS];                     // histogram, or the list of logits that is sorted
+    static_assert(SMP_LIST <= SMP_BINS, "the list shares the histogram's memory");
+    __shared__ float queue[NW][512];
     __shared__ u64 ws[NW];
     __shared__ float wf[NW];
+    __shared__ int wi[2][3 * NW];
     __shared__ u64 found[3];                           // bin, sum before it, sum in it
-    __shared__ int at_found;
+    __shared__ int at_found, listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const T *l = (const T *)a.logits + row * a.ld;
     const int V = a.V;
     const RowSet s = row_set(a, row);
-    auto each8 = [&](auto f) {                         // f(first index, eight cleaned logits); -inf past the end
-        for (int c = tid * 8; c < V; c += NTHR * 8) {
-            f8 v = load8_n(l + c, V - c, -INFINITY);
+    // f(first index, eight logits as they are), called by whole waves: a lane past the end has -inf, and the row's last piece
+    // that is shorter than eight comes as the row's last eight with what was seen before set to -inf.  Four loads are under way before the
+    // first is used (one at a time, a pass over 128000 logits took as long as sixteen trips to the cache).
+    auto each8 = [&](auto f) {
+        typedef typename Vec8<T>::type raw8;
+        constexpr int U = 4, STEP = NTHR * 8;
+        for (int c0 = 0; c0 < V; c0 += U * STEP) {
+            raw8 r[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = clean(v[e]);
-            f(c, v);
+            for (int u = 0; u < U; ++u) {
+                const int c = c0 + u * STEP + tid * 8;
+                if (c < V) r[u] = load8_raw(l + (c + 8 <= V ? c : V - 8));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = c0 + u * STEP + tid * 8;
+                if (__builtin_amdgcn_readfirstlane(c) >= V) break;
+                f8 v = widen<T>(r[u]);
+                if (c + 8 > V) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) if (e < 8 - (V - c)) v[e] = -INFINITY;
+                }
+                f(c + 8 <= V ? c : V - 8, v);
+            }
         }
     };
-    float m = -INFINITY;
-    each8([&](int, const f8 &v) { m = fmaxf(m, max8(v)); });
-    m = team_max<64>(m);
+    float mine = -INFINITY;                            // this lane's largest logit (the maximum passes NaN over)
+    each8([&](int, const f8 &v) { mine = fmaxf(mine, max8(v)); });
+    mine = clean(mine);
+    float m = team_max<64>(mine);
     if (lane == 0) wf[wave] = m;
-    if (tid == 0) at_found = 0x7fffffff;
+    if (tid == 0) { at_found = 0x7fffffff; listed = 0; }
     __syncthreads();
     for (int w = 0; w < NW; ++w) m = fmaxf(m, wf[w]);
     if (m == -INFINITY) { if (tid == 0) a.out[row] = -1; return; }
     if (s.greedy) {
-        int first = 0x7fffffff;
-        each8([&](int c, const f8 &v) {
+        if (mine == m) {
+            int first = 0x7fffffff;
+            each8([&](int c, const f8 &v) {
 #pragma unroll
-            for (int e = 7; e >= 0; --e) if (v[e] == m && c + e < first) first = c + e;
-        });
-        if (first != 0x7fffffff) atomicMin(&at_found, first);
+                for (int e = 7; e >= 0; --e) if (v[e] == m && c + e < first) first = c + e;
+            });
+            atomicMin(&at_found, first);
+        }
         __syncthreads();
         if (tid == 0) a.out[row] = at_found;
         return;
     }
-    const float per_step = (float)(s.it * (double)(SMP_BINS / SMP_RANGE));
+    // an infinite maximum leaves its equals alone: they weigh 1, everything else is below any cut
+    const bool inf = m == INFINITY;
+    const double md = inf ? 0.0 : (double)m;
+    auto weight_raw = [&](float x) { return raw_weight(inf ? (x == m ? 0.f : -INFINITY) : x, md, s.c); };
+    auto weight = [&](float x) -> u64 { return whole_weight(weight_raw(x)); };
+    auto wave_scan = [&](u64 v) {                      // inclusive
+        for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(v, o, 64); if (lane >= o) v += b; }
+        return v;
+    };
+    auto block_before = [&](u64 sum, u64 &total) {     // sum over the lanes before this one
+        const u64 inc = wave_scan(sum);
+        __syncthreads();
+        if (lane == 63) ws[wave] = inc;
+        __syncthreads();
+        u64 before = inc - sum;
+        total = 0;
+        for (int w = 0; w < NW; ++w) { if (w < wave) before += ws[w]; total += ws[w]; }
+        return before;
+    };
+    // The list: (ordered bits, ~index) in hist[0 .. n), sorted to falling logits and rising indices.
+    auto entry = [&](float x, int i) { return (u64)ordered(x) << 32 | (uint32_t)~i; };
+    auto value_of = [&](u64 e) { const uint32_t k = (uint32_t)(e >> 32); return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu)); };
+    auto index_of = [&](u64 e) { return (int)~(uint32_t)e; };
+    auto sort_falling = [&](int n) {
+        __syncthreads();
+        if (n <= (NTHR < 512 ? NTHR : 512)) {          // by counting what is larger (no barriers between steps)
+            const u64 x = tid < n ? hist[tid] : 0;
+            int r = 0;
+            if (tid < n)
+                for (int j = 0; j < n; ++j) { const u64 y = hist[j]; r += y > x || (y == x && j < tid); }
+            __syncthreads();
+            if (tid < n) hist[r] = x;
+            __syncthreads();
+            return;
+        }
+        int n2 = 2;
+        while (n2 < n) n2 *= 2;
+        for (int i = n + tid; i < n2; i += NTHR) hist[i] = 0;
+        for (int k = 2; k <= n2; k *= 2)
+            for (int j = k / 2; j > 0; j /= 2) {
+                __syncthreads();
+                for (int p = tid; p < n2 / 2; p += NTHR) {
+                    const int i = 2 * p - (p & (j - 1));
+                    const u64 x = hist[i], y = hist[i + j];
+                    if ((x < y) == ((i & k) == 0)) { hist[i] = y; hist[i + j] = x; }
+                }
+            }
+        __syncthreads();
+    };
+    auto collect = [&](float from, float to, auto take) {  // logits in [from, to] that `take` wants, in any order; their number (the list may hold fewer)
+        from = fmaxf(from, -FLT_MAX);                  // never -inf: neither drawn nor there (each8)
+        __syncthreads();
+        if (tid == 0) listed = 0;
+        __syncthreads();
+        each8([&](int c, const f8 &v) {
+            if (!(max8(v) >= from)) return;
+            uint32_t hit = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hit |= (v[e] >= from && v[e] <= to ? 1u : 0u) << e;
+            for (; hit; hit &= hit - 1) {              // few
+                const int i = c + __ffs(hit) - 1;
+                const float x = clean((float)l[i]);
+                if (!take(x, i)) continue;
+                const int at = atomicAdd(&listed, 1);
+                if (at < SMP_LIST) hist[at] = entry(x, i);
+            }
+        });
+        __syncthreads();
+        return listed;
+    };
+    // ---- top-k on a short list ---------------------------------------------------------------------------------------
+    if (s.k > 0 && s.k <= NTHR && s.k < V) {
+        // upper bits of the k-th largest of the lanes' maxima, two bits at a time: rounding it down keeps a lower bound
+        const uint32_t key = ordered(mine);
+        uint32_t low = 0;
+        for (int b = 30; b >= 12; b -= 2) {
+            int *buf = wi[(b >> 1) & 1];
+            const int c1 = __popcll(__ballot(key >= (low | 1u << b))), c2 = __popcll(__ballot(key >= (low | 2u << b))), c3 = __popcll(__ballot(key >= (low | 3u << b)));
+            if (lane == 0) { buf[wave] = c1; buf[NW + wave] = c2; buf[2 * NW + wave] = c3; }
+            __syncthreads();
+            int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) { n1 += buf[w]; n2 += buf[NW + w]; n3 += buf[2 * NW + w]; }
+            low |= (n3 >= s.k ? 3u : n2 >= s.k ? 2u : n1 >= s.k ? 1u : 0u) << b;
+        }
+        // as a logit (what lies between -0 and +0 becomes 0, a key below every logit's becomes -inf)
+        float from = low <= 0x007fffffu ? -INFINITY : value_of((u64)low << 32);
+        if (from == 0.f) from = 0.f;
+        const int n = collect(from, INFINITY, [](float, int) { return true; });
+        if (n <= SMP_LIST) {
+            sort_falling(n);
+            const int k = n < s.k ? n : s.k;
+            constexpr int EACH = SMP_LIST / NTHR;      // consecutive entries of a lane
+            u64 w[EACH], e[EACH], sum = 0, total;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                const int i = tid * EACH + q;
+                e[q] = i < k ? hist[i] : 0;
+                const double v = i < k ? weight_raw(value_of(e[q])) : 0.0;
+                w[q] = whole_weight(v);
+                sum += w[q];
+                if (!(v >= s.minw) && i != 0) e[q] = 0;          // fails min-p; its weight still counts for top-p
+            }
+            const u64 before = block_before(sum, total);
+            const u64 goal = s.p < 1.0 ? goal_of(s.p, total) : ~0ull;
+            __syncthreads();
+            u64 run = before;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                const int i = tid * EACH + q;
+                if (i < k) hist[i] = e[q] != 0 && run < goal ? ((u64)(uint32_t)e[q] << 32 | (e[q] >> 32)) : 0;      // ~index first: rising indices
+                run += w[q];
+            }
+            sort_falling(k);                           // by index; what is not kept goes to the end
+            sum = 0;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                const int i = tid * EACH + q;
+                e[q] = i < k ? hist[i] : 0;
+                w[q] = e[q] ? weight(value_of(e[q] << 32)) : 0;
+                sum += w[q];
+            }
+            run = block_before(sum, total);
+            const u64 t = point_of(a.u[row], total);
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                if (run <= t && run + w[q] > t) a.out[row] = index_of(e[q] >> 32);
+                run += w[q];
+            }
+            return;
+        }
+    }
+    // ---- any cut -----------------------------------------------------------------------------------------------------
+    const float per_step = (float)(s.c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE));
     auto step_of = [&](float x) -> int {               // never falls as x falls
         if (x == m) return 0;
         const float q = (m - x) * per_step;
         return q < (float)(SMP_BINS - 1) ? (int)q : SMP_BINS - 1;
     };
-    auto weight = [&](float x) -> u64 {
-        if (x != m && ((double)x - (double)m) * s.it < -(double)SMP_RANGE) return 0;
-        return whole_weight(raw_weight(x, m, s.it));
-    };
-    auto inside = [&](const Cut &c, float x, int i) {
-        const int b = step_of(x);
-        if (b != c.step) return b < c.step;
-        const uint32_t k = ordered(x);
-        return k > c.key || (k == c.key && i <= c.at);
-    };
+    auto inside = [&](const Cut &c, float x, int i) { return x > c.x || (x == c.x && i <= c.at); };
     auto clear = [&]() {
         __syncthreads();
         for (int b = tid; b < SMP_BINS; b += NTHR) hist[b] = 0;
@@ -183,16 +357,11 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // the first bin whose running sum reaches the goal; goal(total) is asked once the total is known
     auto scan = [&](auto goal) {
         __syncthreads();
-        u64 h[PER], sum = 0;
+        u64 h[PER], sum = 0, total;
 #pragma unroll
         for (int q = 0; q < PER; ++q) { h[q] = hist[tid * PER + q]; sum += h[q]; }
-        u64 inc = sum;
-        for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(inc, o, 64); if (lane >= o) inc += b; }
-        if (lane == 63) ws[wave] = inc;
         if (tid == 0) found[0] = SMP_BINS;
-        __syncthreads();
-        u64 total = 0, before = inc - sum;
-        for (int w = 0; w < NW; ++w) { if (w < wave) before += ws[w]; total += ws[w]; }
+        u64 before = block_before(sum, total);
         const u64 want = goal(total);
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
@@ -203,107 +372,144 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         return want;
     };
     // cut where the sum of wt over the elements that `was` keeps reaches its goal
-    auto find_cut = [&](auto was, auto wt, auto goal) {
-        Cut c{SMP_BINS, 0, -1};                        // everything
+    auto find_cut = [&](const Cut &was, auto wt, auto goal) {
         clear();
         each8([&](int i0, const f8 &v) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (v[e] > -INFINITY && was(v[e], i0 + e)) {
+                if (inside(was, v[e], i0 + e)) {
                     const u64 w = wt(v[e]);
                     if (w) atomicAdd(&hist[step_of(v[e])], w);
                 }
         });
         u64 want = scan(goal);
-        if (found[0] == SMP_BINS) return c;            // the goal is not reached: all are kept
-        c.step = (int)found[0];
+        if (found[0] == SMP_BINS) return was;          // the goal is not reached: all are kept
+        const int step = (int)found[0];
+        want -= found[1];
+        // bounds of the step, a little wide, spare most logits the exact test
+        const float wide = (float)step / per_step, far = (float)(step + 1) / per_step, slack = (fabsf(m) + far) * 1e-6f;
+        const float to = m - wide + slack, from = step == SMP_BINS - 1 ? -INFINITY : m - far - slack;
+        const int n = collect(from == from ? from : -INFINITY, to == to ? to : INFINITY, [&](float x, int i) { return inside(was, x, i) && step_of(x) == step; });
+        if (n <= SMP_LIST) {                           // the first of the sorted ones whose running sum reaches what is left
+            sort_falling(n);
+            constexpr int EACH = SMP_LIST / NTHR;
+            u64 w[EACH], sum = 0, total;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) { const int i = tid * EACH + q; w[q] = i < n ? wt(value_of(hist[i])) : 0; sum += w[q]; }
+            u64 run = block_before(sum, total);
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                if (run < want && run + w[q] >= want) found[0] = hist[tid * EACH + q];
+                run += w[q];
+            }
+            __syncthreads();
+            const u64 e = found[0];
+            __syncthreads();
+            return Cut{value_of(e), index_of(e)};
+        }
         uint32_t prefix = 0;
-        for (int shift = 21; found[2] != want - found[1]; shift = shift == 21 ? 10 : 0) {
+        for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
             const int bits = shift == 0 ? 10 : 11;
-            want -= found[1];
             clear();
             each8([&](int i0, const f8 &v) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (v[e] > -INFINITY && step_of(v[e]) == c.step && was(v[e], i0 + e)) {
-                        const uint32_t k = ordered(v[e]);
+                    if (inside(was, v[e], i0 + e) && step_of(v[e]) == step) {
+                        const uint32_t k = ordered(clean(v[e]));
                         if (shift == 21 || (k >> (shift + bits)) == prefix)
                             atomicAdd(&hist[(1 << bits) - 1 - ((k >> shift) & ((1u << bits) - 1))], wt(v[e]));
                     }
             });
             scan([&](u64) { return want; });
             prefix = (prefix << bits) | ((1u << bits) - 1 - (uint32_t)found[0]);
-            c.key = shift ? (prefix << shift) - 1 : prefix;             // while the loop ends here: every key of the prefix is kept
-            if (shift == 0) {
-                // equal logits: as many as it takes, by index
-                if (found[2] == want - found[1]) { c.at = 0x7fffffff; break; }
-                const float x = __uint_as_float(c.key ^ (c.key & 0x80000000u ? 0x80000000u : 0xffffffffu));
-                const u64 w1 = wt(x);
-                u64 need = (want - found[1] + w1 - 1) / w1;             // the need-th of them is the last one kept
-                for (int c0 = 0; c0 < V; c0 += NTHR * 8) {
-                    const int i0 = c0 + tid * 8;
-                    uint32_t hit = 0;
-                    if (i0 < V) {
-                        const f8 v = load8_n(l + i0, V - i0, -INFINITY);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) { const float y = clean(v[e]); if (y == x && was(y, i0 + e)) hit |= 1u << e; }
-                    }
-                    u64 n = __popc(hit), inc = n;
-                    for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(inc, o, 64); if (lane >= o) inc += b; }
-                    __syncthreads();
-                    if (lane == 63) ws[wave] = inc;
-                    __syncthreads();
-                    u64 before = inc - n, all = 0;
-                    for (int w = 0; w < NW; ++w) { if (w < wave) before += ws[w]; all += ws[w]; }
-                    if (before < need && before + n >= need) {
-                        for (u64 q = before + 1; q < need; ++q) hit &= hit - 1;
-                        at_found = i0 + __ffs(hit) - 1;
-                    }
-                    if (all >= need) break;
-                    need -= all;
-                }
-                __syncthreads();
-                c.at = at_found;
-                break;
-            }
+            want -= found[1];
         }
+        // equal logits: as many as it takes, by index
+        const float x = value_of((u64)prefix << 32);
+        const u64 w1 = wt(x);
+        u64 need = (want + w1 - 1) / w1;               // the need-th of them is the last one kept
+        for (int c0 = 0; c0 < V; c0 += NTHR * 8) {
+            const int i0 = c0 + tid * 8;
+            uint32_t hit = 0;
+            if (i0 < V) {
+                const f8 v = load8_n(l + i0, V - i0, -INFINITY);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (v[e] == x && inside(was, v[e], i0 + e)) hit |= 1u << e;
+            }
+            u64 all;
+            const u64 n1 = __popc(hit), before = block_before(n1, all);
+            if (before < need && before + n1 >= need) {
+                for (u64 q = before + 1; q < need; ++q) hit &= hit - 1;
+                at_found = i0 + __ffs(hit) - 1;
+            }
+            if (all >= need) break;
+            need -= all;
+        }
+        __syncthreads();
+        const Cut c{x, at_found};
         __syncthreads();
         return c;
     };
-    Cut ck{SMP_BINS, 0, -1}, cp{SMP_BINS, 0, -1};
-    if (s.k > 0 && s.k < V) ck = find_cut([](float, int) { return true; }, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
-    if (s.p < 1.0) cp = find_cut([&](float x, int i) { return inside(ck, x, i); }, weight, [&](u64 total) { return goal_of(s.p, total); });
-    // the largest logit's lowest index is kept whatever min_p is
-    int top = -1;
-    if (s.minp > 1.0) {
-        if (tid == 0) at_found = 0x7fffffff;
-        __syncthreads();
-        each8([&](int c, const f8 &v) {
+    Cut cut{-INFINITY, -1};                            // everything that can be drawn
+    if (s.k > 0 && s.k < V) cut = find_cut(cut, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
+    if (s.p < 1.0) cut = find_cut(cut, weight, [&](u64 total) { return goal_of(s.p, total); });
+    // min-p is a cut too: the smallest logit that weighs enough, by halving the ordered bit patterns up to the maximum's
+    if (s.minw > 0.0) {
+        uint32_t lo = 0x007fffffu, hi = ordered(m);    // lo: -inf, too light; hi: weighs enough, or is the largest anyway
+        auto enough = [&](uint32_t key) { return weight_raw(value_of((u64)key << 32)) >= s.minw; };
+        const uint32_t near = ordered(clean((float)(md + (log2(s.minw) - SMP_BITS) / s.c)));       // almost always within two patterns
+        if (near > lo + 2 && near + 2 < hi) {
+            if (enough(near + 2)) hi = near + 2;
+            if (!enough(near - 2)) lo = near - 2;
+        }
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (enough(mid)) hi = mid;
+            else lo = mid;
+        }
+        const float x = value_of((u64)hi << 32);
+        int at = 0x7fffffff;
+        if (s.minw > 1099511627776.0) {                // nothing weighs enough: the largest logit's lowest index stays
+            if (tid == 0) at_found = 0x7fffffff;
+            __syncthreads();
+            each8([&](int c, const f8 &v) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) if (v[e] == m) atomicMin(&at_found, c + e);
-        });
-        __syncthreads();
-        top = at_found;
+                for (int e = 0; e < 8; ++e) if (v[e] == m) atomicMin(&at_found, c + e);
+            });
+            __syncthreads();
+            at = at_found;
+        }
+        if (x > cut.x) cut = Cut{x, at};
+        else if (x == cut.x && at < cut.at) cut.at = at;
     }
-    auto kept_weight = [&](float x, int i) -> u64 {
-        if (!(x > -INFINITY) || !inside(ck, x, i) || !inside(cp, x, i)) return 0;
-        if (x != m && ((double)x - (double)m) * s.it < -(double)SMP_RANGE) return 0;
-        const double e = raw_weight(x, m, s.it);
-        return e >= s.minp || i == top ? whole_weight(e) : 0;
-    };
+    auto kept_weight = [&](float x, int i) -> u64 { return weight(inside(cut, x, i) ? x : -INFINITY); };
     const int pieces = (V + 511) / 512;
     __syncthreads();
-    for (int q = wave; q < pieces; q += NW) {          // the wave's pieces of 512 logits
-        const int i0 = q * 512 + lane * 8;
+    // A wave's logits of one step of a pass lie in one piece.  Behind a cut few of them are kept: those are moved together in LDS, so that
+    // 64 lanes weigh 64 kept logits.
+    const bool all = cut.x == -INFINITY;
+    float *q = queue[wave];
+    each8([&](int i0, const f8 &v) {
         u64 sum = 0;
-        if (i0 < V) {
-            const f8 v = load8_n(l + i0, V - i0, -INFINITY);
+        if (all) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += kept_weight(clean(v[e]), i0 + e);
+            for (int e = 0; e < 8; ++e) sum += weight(v[e]);
+        } else {
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool in = inside(cut, v[e], i0 + e);
+                const uint64_t b = __ballot(in);
+                if (in) q[n + __popcll(b & ((1ull << lane) - 1))] = v[e];
+                n += __popcll(b);
+            }
+            wave_fence();
+            for (int j = lane; j < n; j += 64) sum += weight(q[j]);
+            wave_fence();
         }
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if (lane == 0) piece[q] = sum;
-    }
+        if (lane == 0) piece[(i0 + 7) >> 9] = sum;
+    });
     __syncthreads();
     if (wave != 0) return;
     u64 total = 0;
@@ -312,9 +518,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     u64 t = point_of(a.u[row], total);
     int q0 = 0;
     for (;; q0 += 64) {                                // 64 pieces at a time
-        u64 inc = q0 + lane < pieces ? piece[q0 + lane] : 0;
-        const u64 one = inc;
-        for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(inc, o, 64); if (lane >= o) inc += b; }
+        const u64 one = q0 + lane < pieces ? piece[q0 + lane] : 0, inc = wave_scan(one);
         const u64 hit = __ballot(inc > t);
         if (hit) {
             const int w = __ffsll((long long)hit) - 1;
@@ -331,11 +535,9 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         f8 v = splat8(-INFINITY);
         if (i0 < V) v = load8_n(l + i0, V - i0, -INFINITY);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { w8[e] = i0 + e < V ? kept_weight(clean(v[e]), i0 + e) : 0; sum += w8[e]; }
+        for (int e = 0; e < 8; ++e) { w8[e] = kept_weight(v[e], i0 + e); sum += w8[e]; }
     }
-    u64 inc = sum;
-    for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(inc, o, 64); if (lane >= o) inc += b; }
-    const u64 hit = __ballot(inc > t);
+    const u64 inc = wave_scan(sum), hit = __ballot(inc > t);
     if (hit && lane == __ffsll((long long)hit) - 1) {
         u64 run = inc - sum;
         int e = 0;
