@@ -17,7 +17,6 @@ Element types: float32, bfloat16, float16.  All sums and statistics are float32 
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -27,6 +26,8 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _REDUCE = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 _IDS = {torch.int32: 4, torch.int64: 8}
+
+_MOST = 1.7976931348623157e308
 
 Number = Union[int, float]
 
@@ -41,41 +42,55 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-class _on:
-    """The device as current for the call, if it is not already (torch.cuda.device without its cost where nothing changes)."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+def _device(*tensors: Optional[torch.Tensor]) -> int:
+    """Index of the one HIP device that holds the tensors (the checks and errors of ``_lib.require_device``, at a fifth of its time)."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        k = t.get_device()
+        if k < 0 or not t.is_cuda or (index >= 0 and k != index):
+            _lib.require_device(*tensors)
+        index = k
+    return index
 
 
-def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[..., d] as [rows, d] with a contiguous last dimension and one row stride; a copy only where the strides ask for it."""
+def _launch(fn, index: int, what: str, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream, with the device current for the call."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    before = torch._C._cuda_getDevice()
+    if before == index:
+        rc = fn(*args, stream)
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(*args, stream)
+        finally:
+            torch.cuda.set_device(before)
+    if rc != 0:
+        _lib.check(rc, what)
+
+
+def _launch_args(fn, index: int, what: str, layout, *fields) -> None:
+    """The same for the entries that take one argument struct, whose last field is the stream: ``layout`` packs the fields (None is
+    not one of them: 0 stands for NULL)."""
+    _launch(lambda *a: fn(layout.pack(*a)), index, what, *fields)
+
+
+def _rows2d(t: torch.Tensor):
+    """([rows, d] view, row stride) of [..., d]: a contiguous last dimension and one row stride; a copy only where the strides ask for it."""
     d = t.shape[-1]
+    if t.is_contiguous():
+        return (t if t.dim() == 2 else t.view(-1, d) if t.numel() else t.reshape(t.numel() // max(d, 1), d)), d
     if t.dim() != 2:
-        t = t.reshape(-1, d) if d else t.reshape(t.numel(), 0)
-    if t.shape[0] > 1 and t.stride(0) < d or (d > 1 and t.stride(1) != 1):
+        t = t.reshape(-1, d)
+    if (d > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < d):
         t = t.contiguous()
-    return t
+    return t, t.stride(0) if t.shape[0] > 1 else d
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _p(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _p(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _leaf_mark(*tensors: Optional[torch.Tensor]) -> None:
@@ -103,17 +118,14 @@ def _check_ids(ids: torch.Tensor) -> torch.Tensor:
 
 
 def _embed(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
-    lib = _lib.load()
-    dev = _lib.require_device(ids, weight)
-    out = torch.empty(ids.shape + (weight.shape[1],), dtype=weight.dtype, device=dev)
-    if out.numel() == 0:
-        return out
-    w = weight.detach()
-    if w.stride(1) != 1 and w.shape[1] > 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
-        w = w.contiguous()
-    with _on(dev) as stream:
-        _lib.check(lib.dnag_embed_forward(ids.data_ptr(), _IDS[ids.dtype], ids.numel(), w.data_ptr(), _row_stride(w), w.shape[0], w.shape[1],
-                                          _dtype(weight, "weight"), scale, out.data_ptr(), stream), "dnag_embed_forward")
+    index = _device(ids, weight)
+    V, d = weight.shape
+    out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
+    n = ids.numel()
+    if n:
+        w, stride = _rows2d(weight)
+        _launch(_lib.load().dnag_embed_forward, index, "dnag_embed_forward", ids.data_ptr(), _IDS[ids.dtype], n, w.data_ptr(), stride, V, d,
+                _DTYPES[weight.dtype], scale, out.data_ptr())
     return out
 
 
@@ -144,7 +156,7 @@ def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: Number = 1.0
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {weight.shape[0] - 1}")
     if weight.requires_grad and torch.is_grad_enabled():
-        _lib.require_device(ids, weight)
+        _device(ids, weight)
         _leaf_mark(weight)
         return _EmbedTokens.apply(ids, weight, float(scale), padding_idx)
     return _embed(ids, weight, float(scale))
@@ -161,15 +173,14 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
     if num_tokens < 1 or grad.shape[-1] < 1:
         raise ValueError(f"num_tokens={num_tokens}, dim={grad.shape[-1]}: both must be positive")
     code = _dtype(grad, "grad")
-    dev = _lib.require_device(grad, ids)
-    g = _rows2d(grad.detach())
+    index = _device(grad, ids)
+    g, stride = _rows2d(grad)
     rows, d = g.shape
-    out = torch.empty(num_tokens, d, dtype=grad.dtype, device=dev)
+    out = torch.empty((num_tokens, d), dtype=grad.dtype, device=grad.device)
     nbytes = lib.dnag_embed_grad_workspace_bytes(rows, num_tokens, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as stream:
-        _lib.check(lib.dnag_embed_grad(ids.data_ptr(), _IDS[ids.dtype], rows, g.data_ptr(), max(_row_stride(g), d), num_tokens, d, code, float(scale),
-                                       -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _p(ws), nbytes, stream), "dnag_embed_grad")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
+    _launch(lib.dnag_embed_grad, index, "dnag_embed_grad", ids.data_ptr(), _IDS[ids.dtype], rows, g.data_ptr(), stride, num_tokens, d, code, float(scale),
+            -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _p(ws), nbytes)
     return out
 
 
@@ -187,116 +198,115 @@ class BlockNormsGrad(NamedTuple):
     pre_bias: Optional[torch.Tensor]
 
 
+def _small(t: Optional[torch.Tensor], name: str, d: int, dtype) -> Optional[torch.Tensor]:
+    """A norm's weight or bias: [d], the branch's type or float32."""
+    if t is None:
+        return None
+    if t.shape != (d,):
+        raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
+    if t.dtype != dtype and t.dtype != torch.float32:
+        raise ValueError(f"{name} has dtype {t.dtype}; the branch's ({dtype}) or float32 are built")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 class _Seam:
     """The checked arguments of one ``block_norms`` call as the library takes them."""
+    __slots__ = ("index", "shape", "device", "dtype", "x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "rows", "d", "pre", "head",
+                 "arrays")
 
     def __init__(self, x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype=None):
-        if norm not in ("rms", "layer"):
+        layer = norm == "layer"
+        if not layer and norm != "rms":
             raise ValueError(f"norm={norm!r}: 'rms' and 'layer' are built")
         if not eps >= 0:
             raise ValueError(f"eps={eps} must not be negative")
         if x.dim() < 1 or x.shape[-1] < 1:
             raise ValueError(f"x must be [..., dim], got {tuple(x.shape)}")
-        if y is not None and y.shape != x.shape:
-            raise ValueError(f"y {tuple(y.shape)} does not match x {tuple(x.shape)}")
-        if y is None and (gate is not None or post_weight is not None or post_bias is not None):
-            raise ValueError("gate and the norm behind a block need its output y")
-        if y is None and not pre:
-            raise ValueError("without y there is only the norm in front of the next block: pre must be True")
+        if y is None:
+            if gate is not None or post_weight is not None or post_bias is not None:
+                raise ValueError("gate and the norm behind a block need its output y")
+            if not pre:
+                raise ValueError("without y there is only the norm in front of the next block: pre must be True")
+            dtype = dtype or x.dtype
+        else:
+            if y.shape != x.shape:
+                raise ValueError(f"y {tuple(y.shape)} does not match x {tuple(x.shape)}")
+            if dtype is not None and dtype != y.dtype:
+                raise ValueError("dtype is the type of h at the entry (y=None); with y, h has the type of y")
+            dtype = y.dtype
         if not pre and (pre_weight is not None or pre_bias is not None):
             raise ValueError("pre_weight / pre_bias with pre=False")
-        if norm == "rms" and (post_bias is not None or pre_bias is not None):
+        if not layer and (post_bias is not None or pre_bias is not None):
             raise ValueError("RMSNorm has no bias")
-        if dtype is not None and y is not None and dtype != y.dtype:
-            raise ValueError("dtype is the type of h at the entry (y=None); with y, h has the type of y")
+        code, f32 = _DTYPES.get(dtype), torch.float32
+        if code is None:
+            raise ValueError(f"dtype {dtype}; float32, bfloat16 and float16 are built")
+        if x.dtype != dtype and x.dtype != f32:
+            raise ValueError(f"x has dtype {x.dtype}; the branch's ({dtype}) or float32 are built")
         d = x.shape[-1]
-        self.type = y.dtype if y is not None else (dtype or x.dtype)
-        if self.type not in _DTYPES:
-            raise ValueError(f"dtype {self.type}; float32, bfloat16 and float16 are built")
-        if x.dtype not in (self.type, torch.float32):
-            raise ValueError(f"x has dtype {x.dtype}; the branch's ({self.type}) or float32 are built")
         if d > 16384:
             raise ValueError(f"dim={d}: 1 to 16384 are built")
-        self.x, self.y = _rows2d(x.detach()), None if y is None else _rows2d(y.detach())
+        self.x, xs = _rows2d(x)
         rows = self.x.shape[0]
-        self.rows, self.d, self.shape = rows, d, x.shape
-        small, f32 = {}, 0
-        for bit, names in ((2, (("post_weight", post_weight), ("post_bias", post_bias))), (4, (("pre_weight", pre_weight), ("pre_bias", pre_bias)))):
-            have = [t for _, t in names if t is not None]
-            for name, t in names:
-                if t is None:
-                    continue
-                if t.shape != (d,):
-                    raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
-                if t.dtype not in (self.type, torch.float32) or t.dtype != have[0].dtype:
-                    raise ValueError(f"{name} has dtype {t.dtype}; the branch's ({self.type}) or float32 are built, one for a norm's weight and bias")
-                small[name] = t.detach().contiguous()
-            if have and have[0].dtype == torch.float32:
-                f32 |= bit
-        self.gate_rows, self.gate = 1, None
+        self.y, ys = (None, 0) if y is None else _rows2d(y)
+        small = 0
+        self.post_weight, self.post_bias = _small(post_weight, "post_weight", d, dtype), _small(post_bias, "post_bias", d, dtype)
+        self.pre_weight, self.pre_bias = _small(pre_weight, "pre_weight", d, dtype), _small(pre_bias, "pre_bias", d, dtype)
+        for bit, w, b in ((2, post_weight, post_bias), (4, pre_weight, pre_bias)):
+            if w is not None and b is not None and w.dtype != b.dtype:
+                raise ValueError(f"a norm's weight and bias have one type, got {w.dtype} and {b.dtype}")
+            if (w is not None and w.dtype == f32) or (b is not None and b.dtype == f32):
+                small |= bit
+        gate_rows = 1
         if gate is not None:
-            if gate.shape[-1:] != (d,) or gate.dtype not in (self.type, torch.float32):
-                raise ValueError(f"gate must be [..., {d}] of type {self.type} or float32, got {tuple(gate.shape)} {gate.dtype}")
-            self.gate = gate.detach().contiguous()
-            self.gate_rows = gate.numel() // d
-            if self.gate_rows < 1 or rows % self.gate_rows:
-                raise ValueError(f"{rows} rows do not divide into {self.gate_rows} gate rows")
-            if gate.dtype == torch.float32:
-                f32 |= 1
-        self.dev = _lib.require_device(x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
-        a = self.args = _lib.BlockNormsArgsC()
-        a.rows, a.dim, a.gate_rows = rows, d, self.gate_rows
-        a.dtype, a.x_dtype, a.layer_norm, a.pre, a.small_f32 = _DTYPES[self.type], _DTYPES[x.dtype], int(norm == "layer"), int(bool(pre)), f32
-        a.residual_scale, a.eps = float(residual_scale), float(eps)
-        a.x, a.x_stride = self.x.data_ptr(), max(_row_stride(self.x), d)
-        if self.y is not None:
-            a.y, a.y_stride = self.y.data_ptr(), max(_row_stride(self.y), d)
-        a.gate = _p(self.gate)
-        for name, t in small.items():
-            setattr(a, name, t.data_ptr())
-        self.small = small                     # keeps the tensors alive for the call
+            if gate.shape[-1:] != (d,) or (gate.dtype != dtype and gate.dtype != f32):
+                raise ValueError(f"gate must be [..., {d}] of type {dtype} or float32, got {tuple(gate.shape)} {gate.dtype}")
+            gate_rows = gate.numel() // d
+            if gate_rows < 1 or rows % gate_rows:
+                raise ValueError(f"{rows} rows do not divide into {gate_rows} gate rows")
+            if gate.dtype == f32:
+                small |= 1
+            gate = gate if gate.is_contiguous() else gate.contiguous()
+        self.gate = gate
+        self.index = _device(x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+        self.shape, self.device, self.dtype, self.rows, self.d, self.pre = x.shape, x.device, dtype, rows, d, pre
+        self.head = (rows, d, gate_rows, code, _DTYPES[x.dtype], layer, bool(pre), small, float(residual_scale), float(eps))
+        self.arrays = (self.x.data_ptr(), _p(self.y), _p(gate), _p(self.post_weight), _p(self.post_bias), _p(self.pre_weight), _p(self.pre_bias), xs, ys)
 
     def forward(self):
-        a = self.args
-        x_new = torch.empty(self.shape, dtype=self.x.dtype, device=self.dev) if self.y is not None else None
-        h = torch.empty(self.shape, dtype=self.type, device=self.dev) if a.pre else None
+        x_new = torch.empty(self.shape, dtype=self.x.dtype, device=self.device) if self.y is not None else None
+        h = torch.empty(self.shape, dtype=self.dtype, device=self.device) if self.pre else None
         if self.rows:
-            a.x_new, a.h = _p(x_new), _p(h)
-            with _on(self.dev) as a.stream:
-                _lib.check(_lib.load().dnag_block_norms_forward(C.byref(a)), "dnag_block_norms_forward")
+            _launch_args(_lib.load().dnag_block_norms_forward, self.index, "dnag_block_norms_forward", _lib.BLOCK_NORMS_LAYOUT, *self.head, *self.arrays,
+                         _p(x_new), _p(h), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         return x_new, h
 
     def backward(self, grad_x, grad_h, wanted) -> BlockNormsGrad:
-        a, dev = self.args, self.dev
+        gxs = ghs = 0
         if grad_x is not None:
             if grad_x.shape != self.shape or grad_x.dtype != self.x.dtype:
                 raise ValueError(f"grad_x must be {tuple(self.shape)} of type {self.x.dtype}, got {tuple(grad_x.shape)} {grad_x.dtype}")
-            grad_x = _rows2d(grad_x.detach())
-            a.grad_x, a.grad_x_stride = grad_x.data_ptr(), max(_row_stride(grad_x), self.d)
+            grad_x, gxs = _rows2d(grad_x)
         if grad_h is not None:
-            if not a.pre:
+            if not self.pre:
                 raise ValueError("grad_h with pre=False")
-            if grad_h.shape != self.shape or grad_h.dtype != self.type:
-                raise ValueError(f"grad_h must be {tuple(self.shape)} of type {self.type}, got {tuple(grad_h.shape)} {grad_h.dtype}")
-            grad_h = _rows2d(grad_h.detach())
-            a.grad_h, a.grad_h_stride = grad_h.data_ptr(), max(_row_stride(grad_h), self.d)
-        _lib.require_device(self.x, grad_x, grad_h)
+            if grad_h.shape != self.shape or grad_h.dtype != self.dtype:
+                raise ValueError(f"grad_h must be {tuple(self.shape)} of type {self.dtype}, got {tuple(grad_h.shape)} {grad_h.dtype}")
+            grad_h, ghs = _rows2d(grad_h)
+        _device(self.x, grad_x, grad_h)
+        dev, rows = self.device, self.rows
+        new = torch.empty if rows else torch.zeros
         dx = torch.empty(self.shape, dtype=self.x.dtype, device=dev)
-        dy = torch.empty(self.shape, dtype=self.type, device=dev) if self.y is not None else None
-        new = torch.empty if self.rows else torch.zeros
-        grads = {n: new(self.d, dtype=t.dtype, device=dev) for n, t in self.small.items() if n in wanted}
-        dgate = new(self.gate.shape, dtype=self.gate.dtype, device=dev) if self.gate is not None and "gate" in wanted else None
-        if self.rows:
-            a.dx, a.dy, a.d_gate = dx.data_ptr(), _p(dy), _p(dgate)
-            for n, t in grads.items():
-                setattr(a, "d_" + n, t.data_ptr())
+        dy = torch.empty(self.shape, dtype=self.dtype, device=dev) if self.y is not None else None
+        grads = [new(t.shape, dtype=t.dtype, device=dev) if t is not None and n in wanted else None for n, t in
+                 zip(_SMALL, (self.gate, self.post_weight, self.post_bias, self.pre_weight, self.pre_bias))]
+        if rows:
             lib = _lib.load()
-            nbytes = lib.dnag_block_norms_grad_workspace_bytes(C.byref(a))
+            fields = (*self.head, *self.arrays, 0, 0, _p(grad_x), _p(grad_h), gxs, ghs, dx.data_ptr(), _p(dy), *map(_p, grads))
+            nbytes = lib.dnag_block_norms_grad_workspace_bytes(_lib.BLOCK_NORMS_LAYOUT.pack(*fields, 0, 0, 0))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-            with _on(dev) as a.stream:
-                _lib.check(lib.dnag_block_norms_grad(C.byref(a)), "dnag_block_norms_grad")
-        return BlockNormsGrad(dx, dy, dgate, grads.get("post_weight"), grads.get("post_bias"), grads.get("pre_weight"), grads.get("pre_bias"))
+            _launch_args(lib.dnag_block_norms_grad, self.index, "dnag_block_norms_grad", _lib.BLOCK_NORMS_LAYOUT, *fields, ws.data_ptr(), nbytes)
+        return BlockNormsGrad(dx, dy, *grads)
 
 
 _SMALL = ("gate", "post_weight", "post_bias", "pre_weight", "pre_bias")
@@ -383,43 +393,34 @@ class _Distill:
         self.lead = logits.shape[:-1]
         if row_weight is not None and (row_weight.shape != self.lead or row_weight.dtype != torch.float32):
             raise ValueError(f"row_weight must be {tuple(self.lead)} float32, got {tuple(row_weight.shape)} {row_weight.dtype}")
-        self.dev = _lib.require_device(logits, teacher_ids, teacher_logits, row_weight)
-        self.logits = _rows2d(logits.detach())
-        self.kept = (teacher_ids.contiguous(), teacher_logits.detach().contiguous(), None if row_weight is None else row_weight.detach().contiguous())
+        code, tcode = _dtype(logits, "logits"), _dtype(teacher_logits, "teacher_logits")
+        self.index, self.device, self.reduction = _device(logits, teacher_ids, teacher_logits, row_weight), logits.device, reduction
+        self.logits, stride = _rows2d(logits)
         self.rows, self.V = self.logits.shape
-        self.reduction = reduction
-        a = self.args = _lib.DistillArgsC()
-        a.rows, a.vocab, a.logits_stride = self.rows, self.V, max(_row_stride(self.logits), self.V)
-        a.k, a.dtype, a.teacher_dtype = teacher_ids.shape[-1], _dtype(logits, "logits"), _dtype(teacher_logits, "teacher_logits")
-        a.ids_bytes, a.reduction, a.temperature = _IDS[teacher_ids.dtype], _REDUCE[reduction], float(temperature)
-        a.logits, a.teacher_ids, a.teacher_logits, a.row_weight = self.logits.data_ptr(), _p(self.kept[0]), _p(self.kept[1]), _p(self.kept[2])
+        self.kept = (teacher_ids.contiguous(), teacher_logits.contiguous(), None if row_weight is None else row_weight.contiguous())
+        self.head = (self.rows, self.V, stride, teacher_ids.shape[-1], code, tcode, _IDS[teacher_ids.dtype], _REDUCE[reduction], float(temperature),
+                     self.logits.data_ptr(), *map(_p, self.kept))
 
-    def _call(self, fn: str) -> None:
-        a, lib = self.args, _lib.load()
-        nbytes = lib.dnag_distill_workspace_bytes(C.byref(a))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        with _on(self.dev) as a.stream:
-            _lib.check(getattr(lib, fn)(C.byref(a)), fn)
+    def _call(self, fn: str, loss, stats, grad_out, grad) -> None:
+        lib = _lib.load()
+        fields = (*self.head, _p(loss), _p(stats), _p(grad_out), _p(grad))
+        nbytes = lib.dnag_distill_workspace_bytes(_lib.DISTILL_LAYOUT.pack(*fields, 0, 0, 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _launch_args(getattr(lib, fn), self.index, fn, _lib.DISTILL_LAYOUT, *fields, ws.data_ptr(), nbytes)
 
     def loss(self, stats: bool = False, grad: bool = False):
-        a = self.args
         none = self.reduction == "none"
-        loss = (torch.empty if self.rows else torch.zeros)(self.lead if none else (), dtype=torch.float32, device=self.dev)
-        st = torch.empty(self.rows, 2, dtype=torch.float32, device=self.dev) if stats else None
-        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.dev) if grad else None
+        loss = (torch.empty if self.rows else torch.zeros)(self.lead if none else (), dtype=torch.float32, device=self.device)
+        st = torch.empty(self.rows, 2, dtype=torch.float32, device=self.device) if stats else None
+        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.device) if grad else None
         if self.rows:
-            a.loss, a.stats, a.grad = loss.data_ptr(), _p(st), _p(g)
-            self._call("dnag_distill_loss_grad" if grad else "dnag_distill_loss")
+            self._call("dnag_distill_loss_grad" if grad else "dnag_distill_loss", loss, st, None, g)
         return loss, st, g
 
     def backward(self, stats, grad_out):
-        a = self.args
-        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.dev)
+        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.device)
         if self.rows:
-            up = grad_out.detach().to(torch.float32).contiguous()
-            a.stats, a.grad_out, a.grad = stats.data_ptr(), up.data_ptr(), g.data_ptr()
-            self._call("dnag_distill_backward")
+            self._call("dnag_distill_backward", None, stats, grad_out.to(torch.float32).contiguous(), g)
         return g
 
 
@@ -483,28 +484,27 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[N
     lead = logits.shape[:-1]
     if u.shape != lead or u.dtype != torch.float32:
         raise ValueError(f"u must be {tuple(lead)} float32, got {tuple(u.shape)} {u.dtype}")
-    a = _lib.SampleArgsC()
-    a.dtype = _dtype(logits, "logits")
-    kept = []
+    code = _dtype(logits, "logits")
+    numbers, rows = [], []
     for name, value, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                               ("min_p", min_p, torch.float32)):
         if isinstance(value, torch.Tensor):
             if value.shape != lead or value.dtype != kind:
                 raise ValueError(f"{name} must be a number or {tuple(lead)} {kind}, got {tuple(value.shape)} {value.dtype}")
-            value = value.contiguous()
-            kept.append(value)
-            setattr(a, name + "_rows", value.data_ptr())
+            rows.append(value.contiguous())
+            numbers.append(0)
         else:
-            if value != value or value in (float("inf"), float("-inf")):
+            if not -_MOST <= value <= _MOST:
                 raise ValueError(f"{name}={value} must be finite")
-            setattr(a, name, max(-1, min(int(value), 0x7fffffff)) if name == "top_k" else float(value))
-    dev = _lib.require_device(logits, u, *kept)
-    lg = _rows2d(logits.detach())
+            rows.append(None)
+            numbers.append(value)
+    index = _device(logits, u, *rows)
+    lg, stride = _rows2d(logits)
     uc = u.contiguous()
-    out = torch.empty(lead, dtype=torch.int64, device=dev)
-    a.rows, a.vocab, a.logits_stride = lg.shape[0], lg.shape[1], max(_row_stride(lg), lg.shape[1])
-    if a.rows:
-        a.logits, a.u, a.out = lg.data_ptr(), uc.data_ptr(), out.data_ptr()
-        with _on(dev) as a.stream:
-            _lib.check(_lib.load().dnag_sample_tokens(C.byref(a)), "dnag_sample_tokens")
+    out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    n, V = lg.shape
+    if n:
+        t, k, p, q = numbers
+        _launch_args(_lib.load().dnag_sample_tokens, index, "dnag_sample_tokens", _lib.SAMPLE_LAYOUT, n, V, stride, code, max(-1, min(int(k), 0x7fffffff)), t, p, q,
+                     lg.data_ptr(), uc.data_ptr(), *map(_p, rows), out.data_ptr())
     return out
