@@ -21,6 +21,7 @@ struct BnArgs {
     int64_t rows, rpg, G;                              // rows per gate row, gate rows
     int64_t split_rows;                                // backward: rows of one work item (a gate row has S items)
     int S, d, pre, small32;                            // small32: bit 0 gate, bit 1 post norm, bit 2 pre norm are fp32
+    int cell;                                          // backward, rpg < teams of a block: teams that share a run of rows (a power of two, within a wave)
     float rs, eps, inv_d;
 };
 
@@ -116,7 +117,7 @@ template <class TX, class TY, int TPR, int NV, bool LN>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel(const BnArgs a) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1, NA = LN ? 4 : 2;
     __shared__ float red[2][16];
-    __shared__ float comb[NT > 1 ? 256 * 8 * NV : 1];
+    __shared__ __attribute__((aligned(32))) float comb[NT > 1 ? 3 * TPR * 8 * NV : 1];
     RowSum<TPR> sum{red};
     const int lane = threadIdx.x & (TPR - 1), team = threadIdx.x / TPR;
     int n[NV];
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
 #pragma unroll
         for (int k = 0; k < NA; ++k) acc[k][j] = splat8(0.f);
     }
-    auto one_row = [&](int64_t row, size_t g0) {
+    auto one_row = [&](int64_t row, size_t g0) __attribute__((always_inline)) {      // as a call its sums would live in memory
         f8 x[NV], y[NV], gx[NV], gh[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -199,17 +200,25 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
         for (int j = 0; j < NV; ++j)
             if (n[j] > 0) store8_n((TY *)a.dy + row * a.d + (j * TPR + lane) * 8, (gx[j] - t2 - y[j] * t1) * ry, n[j]);
     };
-    // adds the teams' registers in team order; the sum is valid in team 0
+    // adds the teams' registers: within a wave by lane distance, then the block's waves in order; the sum is valid in team 0
     auto join_teams = [&](f8 (&v)[NV]) {
         if constexpr (NT > 1) {
-            __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NV; ++j) *(f8 *)(comb + (size_t)(j * 256 + threadIdx.x) * 8) = v[j];
+            for (int o = TPR; o < 64; o <<= 1)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] += __shfl_xor(v[j][e], o, 64);
+            const int wave = threadIdx.x >> 6;
+            __syncthreads();
+            if (wave > 0 && (threadIdx.x & 63) < TPR)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) *(f8 *)(comb + (size_t)((j * 3 + wave - 1) * TPR + lane) * 8) = v[j];
             __syncthreads();
             if (team == 0)
-                for (int t = 1; t < NT; ++t)
+                for (int w = 0; w < 3; ++w)
 #pragma unroll
-                    for (int j = 0; j < NV; ++j) v[j] += *(const f8 *)(comb + (size_t)(j * 256 + t * TPR + lane) * 8);
+                    for (int j = 0; j < NV; ++j) v[j] += *(const f8 *)(comb + (size_t)((j * 3 + w) * TPR + lane) * 8);
         }
     };
     auto clear = [&]() {
@@ -226,24 +235,27 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
             else store8_n(a.gpart + ((size_t)g * a.S + s) * a.d + c, dg[j], n[j]);
         }
     };
-    if (NT > 1 && a.rpg < NT) {                        // short runs of rows per gate: one team takes a run
-        for (int64_t g = (int64_t)blockIdx.x * NT + team; g < a.G; g += (int64_t)gridDim.x * NT) {
-            clear();
-            for (int64_t r = g * a.rpg; r < (g + 1) * a.rpg; ++r) one_row(r, (size_t)g * a.d);
-            put_gate(g, 0);
-        }
-    } else {                                           // the block takes `split_rows` rows of one gate row at a time
-        for (int64_t w = blockIdx.x; w < a.G * a.S; w += gridDim.x) {
-            const int64_t g = w / a.S;
-            const int s = (int)(w - g * a.S);
-            const int64_t r0 = g * a.rpg + s * a.split_rows, end = (g + 1) * a.rpg, r1 = r0 + a.split_rows < end ? r0 + a.split_rows : end;
-            clear();
-            for (int64_t r = r0 + team; r < r1; r += NT) one_row(r, (size_t)g * a.d);
-            if (a.dgate) {
-                join_teams(dg);
-                if (team == 0) put_gate(g, s);
-            }
-        }
+    // Short runs of rows per gate (fewer than the block has teams): `a.cell` teams of one wave take a run.  Otherwise the block takes
+    // `split_rows` rows of one gate row at a time.
+    const bool few = NT > 1 && a.rpg < NT;
+    const int cells = few ? NT / a.cell : 1, sub = few ? team & (a.cell - 1) : team;
+    const int64_t items = few ? (a.G + cells - 1) / cells : a.G * a.S;
+    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+        const int64_t g = few ? w * cells + team / a.cell : w / a.S;
+        const int s = few ? 0 : (int)(w - g * a.S);
+        const int64_t end = (g + 1) * a.rpg, r0 = g * a.rpg + s * a.split_rows, r1 = few || r0 + a.split_rows > end ? end : r0 + a.split_rows;
+        clear();
+        if (g < a.G)
+            for (int64_t r = r0 + sub; r < r1; r += few ? a.cell : NT) one_row(r, (size_t)g * a.d);
+        if (!a.dgate) continue;
+        if (few) {
+            for (int o = TPR; o < a.cell * TPR; o <<= 1)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dg[j][e] += __shfl_xor(dg[j][e], o, 64);
+        } else join_teams(dg);
+        if (sub == 0 && g < a.G) put_gate(g, s);
     }
     if (!a.part) return;
 #pragma unroll
@@ -301,19 +313,26 @@ int lanes_for(int64_t d) {                             // lanes of a team: eight
     const int64_t v = ceil_div(d, 8);
     return v <= 8 ? 8 : v <= 32 ? 32 : pow2_at_least(v, 64, 1024);
 }
+#ifndef BNG
+#define BNG 256
+#endif
+int grad_lanes_for(int64_t d) { return d > 1024 && d <= 2048 ? BNG : lanes_for(d); }
 struct BnPlan {
-    int tpr, nt, nblk, S, na;
+    int tpr, nt, nblk, S, na, cell;
     int64_t split;
     size_t gpart, bytes;
 };
 BnPlan grad_plan(const dnag_block_norms_args &p) {
     BnPlan q;
-    q.tpr = lanes_for(p.dim);
+    q.tpr = grad_lanes_for(p.dim);
     q.nt = q.tpr <= 64 ? 256 / q.tpr : 1;
     q.na = p.layer_norm ? 4 : 2;
     const int64_t G = p.gate_rows, rpg = p.rows / G;
     // two blocks of 256 lanes for every CU: fewer partial sums than a block per row, and enough rows in flight
-    const int64_t target = q.tpr <= 256 ? 1024 : q.tpr == 512 ? 512 : 256;
+#ifndef BNT
+#define BNT 1024
+#endif
+    const int64_t target = q.tpr <= 64 ? 512 : q.tpr <= 256 ? BNT : q.tpr == 512 ? 512 : 256;
     q.S = 1;
     if (rpg >= q.nt) {
         int64_t s = ceil_div(target, G), most = ceil_div(rpg, q.nt);
@@ -321,7 +340,11 @@ BnPlan grad_plan(const dnag_block_norms_args &p) {
         q.split = ceil_div(rpg, s);
         q.S = (int)ceil_div(rpg, q.split);
     } else q.split = rpg;
-    const int64_t items = rpg >= q.nt ? G * q.S : ceil_div(G, q.nt);
+    // a run of rows shared by as many teams of a wave as it has rows: one team for a run left the chip half empty (4096 runs of
+    // 8 rows of 64: 36 us; shared by 8 teams: 17)
+    q.cell = 1;
+    while (q.cell * 2 <= rpg && q.cell * 2 * q.tpr <= 64) q.cell *= 2;
+    const int64_t items = rpg >= q.nt ? G * q.S : ceil_div(G, q.nt / q.cell);
     q.nblk = (int)(items < target ? items : target);
     q.gpart = align256((size_t)q.nblk * q.na * p.dim * 4);
     q.bytes = q.gpart + (q.S > 1 ? (size_t)G * q.S * p.dim * 4 : 0);
@@ -360,8 +383,14 @@ void launch_width(const BnArgs &a, int tpr, bool grad, unsigned blocks, hipStrea
     switch (tpr) {
         case 8: launch<TX, TY, 8, 1, LN>(a, grad, blocks, st); break;
         case 32: launch<TX, TY, 32, 1, LN>(a, grad, blocks, st); break;
-        case 64: launch<TX, TY, 64, 1, LN>(a, grad, blocks, st); break;
-        case 128: launch<TX, TY, 128, 1, LN>(a, grad, blocks, st); break;
+        case 64:
+            if (a.d > 512) launch<TX, TY, 64, 4, LN>(a, grad, blocks, st);
+            else launch<TX, TY, 64, 1, LN>(a, grad, blocks, st);
+            break;
+        case 128:
+            if (a.d > 1024) launch<TX, TY, 128, 2, LN>(a, grad, blocks, st);
+            else launch<TX, TY, 128, 1, LN>(a, grad, blocks, st);
+            break;
         case 256: launch<TX, TY, 256, 1, LN>(a, grad, blocks, st); break;
         case 512: launch<TX, TY, 512, 1, LN>(a, grad, blocks, st); break;
         default:
@@ -414,7 +443,7 @@ extern "C" int dnag_block_norms_grad(const dnag_block_norms_args *p) {
     BnArgs a = common_args(*p);
     a.gx = p->grad_x; a.gh = p->grad_h; a.gxs = p->grad_x_stride; a.ghs = p->grad_h_stride;
     a.dx = p->dx; a.dy = p->dy; a.dgate = p->d_gate;
-    a.S = q.S; a.split_rows = q.split;
+    a.S = q.S; a.split_rows = q.split; a.cell = q.cell;
     const bool weights = p->d_post_weight || p->d_post_bias || p->d_pre_weight || p->d_pre_bias;
     a.part = weights ? (float *)p->workspace : nullptr;
     a.gpart = (float *)((char *)p->workspace + q.gpart);

@@ -30,27 +30,6 @@ struct DistillArgs {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <int TPR> struct TeamRed {
-    float *red;                                        // [2][16], TPR > 64
-    int turn = 0;
-    template <class F> __device__ __forceinline__ float all(float v, F f) {
-#pragma unroll
-        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
-        if constexpr (TPR > 64) {
-            float *b = red + 16 * turn;
-            turn ^= 1;
-            if ((threadIdx.x & 63) == 0) b[threadIdx.x >> 6] = v;
-            __syncthreads();
-            v = b[0];
-#pragma unroll
-            for (int w = 1; w < TPR / 64; ++w) v = f(v, b[w]);
-        }
-        return v;
-    }
-};
-struct AddF { __device__ float operator()(float a, float b) const { return a + b; } };
-struct MaxF { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-
 // MODE 0: loss (and stats), 1: loss and gradient, 2: gradient from stats and the upstream gradient
 template <class T, int TPR, int NV, int MODE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const DistillArgs a) {
@@ -59,10 +38,9 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const Di
     constexpr float LOW = -3.0e38f;                    // below every logit that counts: -inf - LOW = -inf, exp2 = 0
     typedef typename Vec8<T>::type raw8;
     extern __shared__ char lds[];
-    __shared__ float red[32];
+    __shared__ float red[33];                          // pairs of the waves; [32]: the teacher's maximum
     float *tp = (float *)lds + (size_t)(threadIdx.x / TPR) * 2 * a.K;      // the team's entries: probability, index
     int *ti = (int *)(tp + a.K);
-    TeamRed<TPR> team{red};
     const int lane = threadIdx.x & (TPR - 1);
     const int64_t row = (int64_t)blockIdx.x * NT + threadIdx.x / TPR;
     if (row >= a.rows) return;
@@ -111,42 +89,57 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const Di
 #pragma unroll
             for (int o = TW / 2; o > 0; o >>= 1) tsum += __shfl_xor(tsum, o, 64);
         }
-        if constexpr (TPR > 64) if (lane == 0) red[31] = tmax;
+        if constexpr (TPR > 64) if (lane == 0) red[32] = tmax;
     }
-    if constexpr (TPR > 64) { __syncthreads(); tmax = red[31]; }
+    if constexpr (TPR > 64) { __syncthreads(); tmax = red[32]; }
     if (tmax == -INFINITY) { zero_row(); return; }     // no entry (the same for the whole team)
-    float m, sum;
+    // Every lane takes its exponentials relative to its own largest logit `tm`, in fp32 (MODE 1 keeps them for the gradient), so that one
+    // exchange of (maximum, sum) pairs gives the row's: exp(s - m) = exp(s - tm) exp(tm - m).
+    float m, sum, tm = LOW, own = 0.f;
+    constexpr bool KEEP = MODE == 1 && NV > 0 && NV <= 8;      // 16 pieces: their registers would spill
+    f8 ex[KEEP ? NV : 1];
     if constexpr (MODE == 2) { m = a.stats[2 * row]; sum = a.stats[2 * row + 1]; }
-    else if constexpr (NV > 0) {
-        m = LOW;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) m = fmaxf(m, max8(widen<T>(x[j])));
-        if constexpr (TPR > 64) __syncthreads();       // red[31] is read; the buffers of `team` overlap it
-        m = team.all(m, MaxF());
-        sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            f8 v = (widen<T>(x[j]) - m) * a.c2;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = exp2_hw(v[e]);
-            sum += sum8(v);
-        }
-        sum = team.all(sum, AddF());
-    } else {
-        float tm = LOW, ts = 0.f;
-        for (int c = lane * 8; c < a.V; c += TPR * 8) {
-            f8 v = load8_n(s + c, a.V - c, -INFINITY);
-            const float nm = fmaxf(tm, max8(v));
-            ts *= exp2_hw((tm - nm) * a.c2);
-            tm = nm;
+    else {
+        auto exps = [&](f8 v) {
             v = (v - tm) * a.c2;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = exp2_hw(v[e]);
-            ts += sum8(v);
+            return v;
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) tm = fmaxf(tm, max8(widen<T>(x[j])));
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const f8 v = exps(widen<T>(x[j]));
+                own += sum8(v);
+                if constexpr (KEEP) ex[j] = v;
+            }
+        } else
+            for (int c = lane * 8; c < a.V; c += TPR * 8) {
+                const f8 v = load8_n(s + c, a.V - c, -INFINITY);
+                const float nm = fmaxf(tm, max8(v));
+                own *= exp2_hw((tm - nm) * a.c2);
+                tm = nm;
+                own += sum8(exps(v));
+            }
+        m = tm;
+#pragma unroll
+        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        sum = own * exp2_hw((tm - m) * a.c2);
+#pragma unroll
+        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if constexpr (TPR > 64) {
+            if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = m; red[2 * (threadIdx.x >> 6) + 1] = sum; }
+            __syncthreads();
+            float all = red[0];
+#pragma unroll
+            for (int w = 1; w < TPR / 64; ++w) all = fmaxf(all, red[2 * w]);
+            m = all;
+            sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < TPR / 64; ++w) sum += red[2 * w + 1] * exp2_hw((red[2 * w] - m) * a.c2);
         }
-        if constexpr (TPR > 64) __syncthreads();
-        m = team.all(tm, MaxF());
-        sum = team.all(ts * exp2_hw((tm - m) * a.c2), AddF());
     }
     if constexpr (MODE < 2) {
         if (lane < TW) {
@@ -176,7 +169,14 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const Di
             for (int e = 0; e < 8; ++e) v[e] = exp2_hw(v[e]);
             store8_n(g + c, v * fq, a.V - c);
         };
-        if constexpr (NV > 0) {
+        if constexpr (KEEP) {
+            const float ft = fq * exp2_hw((tm - m) * a.c2);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * TPR + lane) * 8;
+                if (c < a.V) store8_n(g + c, ex[j] * ft, a.V - c);
+            }
+        } else if constexpr (NV > 0) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * TPR + lane) * 8;

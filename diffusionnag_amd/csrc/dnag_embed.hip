@@ -199,21 +199,25 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict_
     }
 }
 
-// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` entries.
+// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` (at most TPR, or 64) entries.  The lanes fetch the
+// entries at once, one each, so that the rows' addresses are known before the first row is asked for; eight rows are
+// under way at a time (fetching four entries, then their rows, in turn: 94 us for 32768 x 2048 bf16; this: 41).
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t rows,
                                                         const T *__restrict__ grad, int64_t gstride, uint32_t V, int d, float scale, int chunk, int ntile,
                                                         T *__restrict__ out, uint32_t *__restrict__ begin, uint32_t *__restrict__ last, float *__restrict__ part) {
+    typedef typename Vec8<T>::type raw8;
     const int lane = threadIdx.x & (TPR - 1);
     const int64_t unit = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const int64_t ch = unit / ntile;
     const int tile = (int)(unit - ch * ntile);
     const int64_t i0 = ch * chunk, i1 = i0 + chunk < rows ? i0 + chunk : rows;
-    if (i0 >= rows) return;
+    if (i0 >= rows) return;                            // whole teams
     const int c = (tile * TPR + lane) * 8, n = d - c < 8 ? d - c : 8;
     f8 acc = splat8(0.f);
     uint32_t cur = key[i0];
     bool older = i0 > 0 && key[i0 - 1] == cur;          // the token's rows began in an earlier chunk
+    const uint32_t next = i1 < rows ? key[i1] : ~0u;
     int64_t start = i0;
     auto flush = [&](int64_t end, bool more) {          // rows start .. end - 1 belong to `cur`; more: they go on in the next chunk
         if (tile == 0 && lane == 0) {
@@ -224,34 +228,39 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restri
         if (!older && !more) store8_n(out + (size_t)cur * d + c, acc * scale, n);
         else store8_n(part + ((size_t)ch * 2 + (older ? 0 : 1)) * d + c, acc, n);
     };
-    for (int64_t i = i0; i < i1 && cur < V; i += 4) {
-        uint32_t k[4], p[4];
-        f8 x[4];
+    for (int64_t b = i0; b < i1; b += TPR) {            // entries b .. b + TPR - 1, one per lane
+        const int64_t mine = b + lane < i1 ? b + lane : i1 - 1;
+        const uint32_t kk = key[mine], pp = pos[mine];
+        const int m = (int)(i1 - b < TPR ? i1 - b : TPR);
+        for (int g = 0; g < m; g += 8) {
+            uint32_t k[8];
+            raw8 x[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t ii = i + u < i1 ? i + u : i1 - 1;
-            k[u] = key[ii];
-            p[u] = pos[ii];
-        }
+            for (int u = 0; u < 8; ++u) {
+                const int src = g + u < m ? g + u : m - 1;
+                k[u] = g + u < m ? __shfl(kk, src, TPR) : cur;
+                const T *p = grad + (size_t)__shfl(pp, src, TPR) * gstride + c;
+                if (n == 8) x[u] = load8_raw(p);
+                else
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            x[u] = splat8(0.f);
-            if (n > 0) x[u] = load8_n(grad + (size_t)p[u] * gstride + c, n);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u < i1) {
-                if (k[u] != cur) {
-                    if (cur < V) flush(i + u, false);
-                    acc = splat8(0.f);
-                    cur = k[u];
-                    older = false;
-                    start = i + u;
-                }
-                acc += x[u];
+                    for (int e = 0; e < 8; ++e) x[u][e] = e < n ? p[e] : (T)0.f;
             }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (g + u < m) {
+                    if (k[u] != cur) {
+                        if (cur < V) flush(b + g + u, false);
+                        acc = splat8(0.f);
+                        cur = k[u];
+                        older = false;
+                        start = b + g + u;
+                    }
+                    acc += widen<T>(x[u]);
+                }
+            if (cur >= V) return;                       // the dropped ones are the list's end
+        }
     }
-    if (cur < V) flush(i1, i1 < rows && key[i1] == cur);
+    if (cur < V) flush(i1, next == cur);
 }
 
 // Tokens whose rows cross chunk borders: their pieces in chunk order.  Tokens without rows: zeros.  (The rest is written.)
@@ -262,14 +271,17 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t *__restr
     __shared__ float sh[256 * 8];
     const int cl = threadIdx.x & (cols - 1), share = threadIdx.x / cols, shares = 256 / cols;      // cols: a power of two
     const int64_t v0 = (int64_t)blockIdx.x * per_block, v1 = v0 + per_block < V ? v0 + per_block : V;
+    __shared__ uint32_t ends[64], starts[64];
+    if (threadIdx.x < v1 - v0) { ends[threadIdx.x] = last[v0 + threadIdx.x]; starts[threadIdx.x] = begin[v0 + threadIdx.x]; }
+    __syncthreads();
     for (int64_t v = v0; v < v1; ++v) {                // the same for the whole block
-        const uint32_t e = last[v];
+        const uint32_t e = ends[v - v0];
         T *dst = out + (size_t)v * d;
         if (e == 0) {
             for (int c = threadIdx.x * 8; c < d; c += 2048) store8_n(dst + c, splat8(0.f), d - c < 8 ? d - c : 8);
             continue;
         }
-        const uint32_t c0 = begin[v] / chunk, c1 = (e - 1) / chunk;
+        const uint32_t c0 = starts[v - v0] / chunk, c1 = (e - 1) / chunk;
         if (c0 == c1) continue;
         const uint32_t count = c1 - c0 + 1, each = (count + shares - 1) / shares;
         const uint32_t a = share * each, b = a + each < count ? a + each : count;
@@ -317,8 +329,8 @@ GradPlan grad_plan(int64_t rows, int64_t V, int64_t d) {
     }
     p.lds = rows <= EMB_SORT_LDS;
     const int64_t wide = ceil_div(d, 512);
-    p.chunk = 64;
-    while (p.chunk > 16 && ceil_div(rows, p.chunk) * wide < 2048) p.chunk /= 2;
+    p.chunk = 64;                      // fewer pieces, but no fewer waves than eight for each of 256 CUs
+    while (p.chunk > 8 && ceil_div(rows, p.chunk) * wide < 4096) p.chunk /= 2;
     p.nchunk = (int)ceil_div(rows, p.chunk);
     if (!p.lds) {
         p.per_block = ceil_div(ceil_div(rows, EMB_MAXB), 256) * 256;
