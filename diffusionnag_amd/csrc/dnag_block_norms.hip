@@ -74,15 +74,21 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_kernel(cons
     if (row >= a.rows) return;                         // whole teams; TPR > 64: the block has one team
     int n[NV];
     f8 x[NV], y[NV];
+    typename Vec8<TX>::type rx[NV];
+    typename Vec8<TY>::type ry[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = (j * TPR + lane) * 8;
         n[j] = a.d - c;
-        x[j] = y[j] = splat8(0.f);
         if (n[j] > 0) {
-            x[j] = load8_n((const TX *)a.x + row * a.xs + c, n[j]);
-            if (a.y) y[j] = load8_n((const TY *)a.y + row * a.ys + c, n[j]);
+            rx[j] = load8_raw_n((const TX *)a.x + row * a.xs + c, n[j]);
+            if (a.y) ry[j] = load8_raw_n((const TY *)a.y + row * a.ys + c, n[j]);
         }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        x[j] = n[j] > 0 ? widen<TX>(rx[j]) : splat8(0.f);
+        y[j] = n[j] > 0 && a.y ? widen<TY>(ry[j]) : splat8(0.f);
     }
     if (a.y) {
         normalise<LN>(y, n, sum, a.eps, a.inv_d);
@@ -130,16 +136,24 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
     }
     auto one_row = [&](int64_t row, size_t g0) __attribute__((always_inline)) {      // as a call its sums would live in memory
         f8 x[NV], y[NV], gx[NV], gh[NV];
+        typename Vec8<TX>::type rx[NV], rgx[NV];
+        typename Vec8<TY>::type ry_[NV], rgh[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * TPR + lane) * 8;
-            x[j] = y[j] = gx[j] = gh[j] = splat8(0.f);
             if (n[j] > 0) {
-                x[j] = load8_n((const TX *)a.x + row * a.xs + c, n[j]);
-                if (a.y) y[j] = load8_n((const TY *)a.y + row * a.ys + c, n[j]);
-                if (a.gx) gx[j] = load8_n((const TX *)a.gx + row * a.gxs + c, n[j]);
-                if (a.gh) gh[j] = load8_n((const TY *)a.gh + row * a.ghs + c, n[j]);
+                rx[j] = load8_raw_n((const TX *)a.x + row * a.xs + c, n[j]);
+                if (a.y) ry_[j] = load8_raw_n((const TY *)a.y + row * a.ys + c, n[j]);
+                if (a.gx) rgx[j] = load8_raw_n((const TX *)a.gx + row * a.gxs + c, n[j]);
+                if (a.gh) rgh[j] = load8_raw_n((const TY *)a.gh + row * a.ghs + c, n[j]);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            x[j] = n[j] > 0 ? widen<TX>(rx[j]) : splat8(0.f);
+            y[j] = n[j] > 0 && a.y ? widen<TY>(ry_[j]) : splat8(0.f);
+            gx[j] = n[j] > 0 && a.gx ? widen<TX>(rgx[j]) : splat8(0.f);
+            gh[j] = n[j] > 0 && a.gh ? widen<TY>(rgh[j]) : splat8(0.f);
         }
         auto small = [&](const void *p, int bit, size_t at, int j, float none) {
             return p && n[j] > 0 ? load8_either<TY>(p, a.small32 & bit, at, n[j]) : splat8(none);
@@ -291,9 +305,7 @@ __global__ __launch_bounds__(1024) void block_norms_join_kernel(const BnJoin a) 
     const size_t step = weight ? (size_t)a.na * a.d : (size_t)a.d;
     const int per = (count + 15) / 16, k0 = w * per, k1 = k0 + per < count ? k0 + per : count;
     float s = 0.f;
-    if (c < a.d)
-#pragma unroll 8
-        for (int k = k0; k < k1; ++k) s += src[k * step + c];
+    if (c < a.d) s = sum_strided(src + c, k0, k1, step);
     q[w][col] = s;
     __syncthreads();
     if (w != 0 || c >= a.d) return;

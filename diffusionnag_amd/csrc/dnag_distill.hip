@@ -32,7 +32,8 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 
 // MODE 0: loss (and stats), 1: loss and gradient, 2: gradient from stats and the upstream gradient
 template <class T, int TPR, int NV, int MODE>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
+(const DistillArgs a) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1, TW = TPR < 64 ? TPR : 64;      // TW: lanes that handle the teacher's entries
     constexpr int NR = NV > 0 ? NV : 1;
     constexpr float LOW = -3.0e38f;                    // below every logit that counts: -inf - LOW = -inf, exp2 = 0
@@ -203,7 +204,13 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel(const Di
 __global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ w, int64_t rows, float *__restrict__ out) {
     __shared__ float q[16];
     float s = 0.f;
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) s += w[i] > 0.f ? w[i] : 0.f;
+    for (int64_t i = threadIdx.x; i < rows; i += 8192) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { const int64_t q = i + u * 1024; x[u] = w[q < rows ? q : i]; if (!(q < rows && x[u] > 0.f)) x[u] = 0.f; }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += x[u];
+    }
     s = team_sum<64>(s);
     if ((threadIdx.x & 63) == 0) q[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -216,8 +223,13 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const float *__restr
                                                             float *__restrict__ out) {
     __shared__ float q[16];
     float s = 0.f;
-#pragma unroll 8
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) s += row_loss[i];
+    for (int64_t i = threadIdx.x; i < rows; i += 8192) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { const int64_t q = i + u * 1024; x[u] = row_loss[q < rows ? q : i]; }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += i + u * 1024 < rows ? x[u] : 0.f;
+    }
     s = team_sum<64>(s);
     if ((threadIdx.x & 63) == 0) q[threadIdx.x >> 6] = s;
     __syncthreads();

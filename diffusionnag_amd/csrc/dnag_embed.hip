@@ -55,17 +55,17 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const I *__restrict__ id
     const int64_t len = (b1 - b0 + 31) / 32, t0 = b0 + team * len, t1 = t0 + len < b1 ? t0 + len : b1;
     if (n > 0)
         for (int64_t t = t0; t < t1; t += 4) {
-            f8 x[4];
+            typename Vec8<T>::type x[4];
             uint32_t k[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int64_t tt = t + u < t1 ? t + u : t1 - 1;
                 k[u] = t + u < t1 ? emb_key(ids, tt, V, pad) : (uint32_t)V;
-                x[u] = load8_n(grad + tt * gstride + c, n);
+                x[u] = load8_raw_n(grad + tt * gstride + c, n);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (k[u] < (uint32_t)V) *(f8 *)(mine + k[u] * 64) += x[u];
+                if (k[u] < (uint32_t)V) *(f8 *)(mine + k[u] * 64) += widen<T>(x[u]);
         }
     __syncthreads();
     for (int i = threadIdx.x; i < V * 64; i += 256) {
@@ -85,9 +85,7 @@ __global__ __launch_bounds__(1024) void embed_few_join_kernel(const float *__res
     const int64_t i = (int64_t)blockIdx.x * 64 + col;
     const int per = (nblk + 15) / 16, a = w * per, b = a + per < nblk ? a + per : nblk;
     float s = 0.f;
-    if (i < n)
-#pragma unroll 8
-        for (int k = a; k < b; ++k) s += part[(size_t)k * n + i];
+    if (i < n) s = sum_strided(part + i, a, b, (size_t)n);
     q[w][col] = s;
     __syncthreads();
     if (w == 0 && i < n) {
@@ -122,6 +120,32 @@ __global__ __launch_bounds__(1024) void embed_sort_lds_kernel(const I *__restric
     for (int i = threadIdx.x; i < rows; i += 1024) { key[i] = (uint32_t)(pr[i] >> 32); pos[i] = (uint32_t)pr[i]; }
 }
 
+// Rows of tokens that do not occur, written by workgroups that ride along with the sort's launches (those keep 32 of 256 CUs
+// busy): tokens [v0, v1) whose `last` is 0, `units` 16-bit words each.
+struct EmbFill {
+    const uint32_t *last;
+    uint16_t *out;
+    int64_t v0, v1, units;
+    int first;                         // workgroups of the sort itself
+};
+__device__ __forceinline__ void emb_fill(const EmbFill &f) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    const int64_t wgs = gridDim.x - f.first;
+    for (int64_t b = f.v0 + (blockIdx.x - f.first); b < f.v1; b += 64 * wgs) {       // 64 tokens at a time, a lane asks for each
+        const int64_t mine = b + (threadIdx.x & 63) * wgs;
+        uint64_t empty = __ballot(mine < f.v1 && f.last[mine < f.v1 ? mine : b] == 0);       // the same in every wave
+        for (; empty; empty &= empty - 1) {
+            uint16_t *dst = f.out + (b + (__ffsll((long long)empty) - 1) * wgs) * f.units;
+            for (int64_t c = threadIdx.x * 8; c < f.units; c += blockDim.x * 8) {
+                if (f.units - c >= 8) __builtin_memcpy(dst + c, &zero, 16);
+                else
+                    for (int64_t e = c; e < f.units; ++e) dst[e] = 0;
+            }
+        }
+    }
+}
+
 // Stable radix sort, digits of eight bits.  A block owns a contiguous range of the list and each of its four waves a
 // contiguous quarter; at most EMB_MAXB blocks, so that every block sums the others' histograms by itself (no scan launch).
 #define EMB_MAXB 128
@@ -131,27 +155,30 @@ __device__ __forceinline__ uint32_t emb_pass_key(const I *ids, const uint32_t *k
 }
 template <class I>
 __global__ __launch_bounds__(256) void embed_hist_kernel(const I *__restrict__ ids, const uint32_t *__restrict__ kin, int64_t rows, int64_t per_block,
-                                                         int64_t V, int64_t pad, int shift, uint32_t *__restrict__ hist, uint32_t *__restrict__ last) {
+                                                         int64_t V, int64_t pad, int shift, uint32_t *__restrict__ hist, uint32_t *__restrict__ last, EmbFill fill) {
+    if ((int)blockIdx.x >= fill.first) { emb_fill(fill); return; }
     __shared__ uint32_t h[256];
     h[threadIdx.x] = 0;
     __syncthreads();
     const int64_t b0 = blockIdx.x * per_block, b1 = b0 + per_block < rows ? b0 + per_block : rows;
     for (int64_t i = b0 + threadIdx.x; i < b1; i += 256) atomicAdd(&h[(emb_pass_key(ids, kin, i, V, pad) >> shift) & 255], 1u);   // counts: any order
     if (last)
-        for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < V; v += (int64_t)gridDim.x * 256) last[v] = 0;
+        for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < V; v += (int64_t)fill.first * 256) last[v] = 0;
     __syncthreads();
     hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
 }
 template <class I>
 __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict__ ids, const uint32_t *__restrict__ kin, const uint32_t *__restrict__ pin,
                                                             int64_t rows, int64_t per_block, int64_t V, int64_t pad, int shift,
-                                                            const uint32_t *__restrict__ hist, uint32_t *__restrict__ kout, uint32_t *__restrict__ pout) {
+                                                            const uint32_t *__restrict__ hist, uint32_t *__restrict__ kout, uint32_t *__restrict__ pout,
+                                                            uint32_t *__restrict__ mark, EmbFill fill) {
+    if ((int)blockIdx.x >= fill.first) { emb_fill(fill); return; }
     __shared__ uint32_t cnt[4][256], scan[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // base of digit tid for this block: digits before it in the whole list, then the same digit in earlier blocks
     uint32_t total = 0, before = 0;
 #pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; ++b) {
+    for (int b = 0; b < fill.first; ++b) {
         const uint32_t x = hist[b * 256 + tid];
         total += x;
         before += b < (int)blockIdx.x ? x : 0;
@@ -193,6 +220,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict_
         if (on) {
             kout[first + rank] = k;
             pout[first + rank] = pin ? pin[i] : (uint32_t)i;
+            if (mark && k < (uint32_t)V) mark[k] = ~0u;          // the token occurs (any order, one value)
             if (rank == 0) cnt[wave][dig] = first + (uint32_t)__popcll(same);
         }
         wave_fence();
@@ -205,25 +233,22 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict_
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t rows,
                                                         const T *__restrict__ grad, int64_t gstride, uint32_t V, int d, float scale, int chunk, int ntile,
-                                                        T *__restrict__ out, uint32_t *__restrict__ begin, uint32_t *__restrict__ last, float *__restrict__ part) {
+                                                        T *__restrict__ out, uint32_t *__restrict__ last, float *__restrict__ part) {
     typedef typename Vec8<T>::type raw8;
     const int lane = threadIdx.x & (TPR - 1);
-    const int64_t unit = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int in_block = TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / TPR;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / TPR) + in_block;
     const int64_t ch = unit / ntile;
     const int tile = (int)(unit - ch * ntile);
     const int64_t i0 = ch * chunk, i1 = i0 + chunk < rows ? i0 + chunk : rows;
     if (i0 >= rows) return;                            // whole teams
     const int c = (tile * TPR + lane) * 8, n = d - c < 8 ? d - c : 8;
     f8 acc = splat8(0.f);
-    uint32_t cur = key[i0];
+    uint32_t cur = TPR == 64 ? __builtin_amdgcn_readfirstlane(key[i0]) : key[i0];
     bool older = i0 > 0 && key[i0 - 1] == cur;          // the token's rows began in an earlier chunk
     const uint32_t next = i1 < rows ? key[i1] : ~0u;
-    int64_t start = i0;
-    auto flush = [&](int64_t end, bool more) {          // rows start .. end - 1 belong to `cur`; more: they go on in the next chunk
-        if (tile == 0 && lane == 0) {
-            if (!older) begin[cur] = (uint32_t)start;
-            if (!more) last[cur] = (uint32_t)end;
-        }
+    auto flush = [&](int64_t end, bool more) {          // the rows of `cur` before `end`; more: they go on in the next chunk
+        if (tile == 0 && lane == 0 && !more) last[cur] = (uint32_t)end;
         if (n <= 0) return;
         if (!older && !more) store8_n(out + (size_t)cur * d + c, acc * scale, n);
         else store8_n(part + ((size_t)ch * 2 + (older ? 0 : 1)) * d + c, acc, n);
@@ -238,12 +263,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restri
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int src = g + u < m ? g + u : m - 1;
-                k[u] = g + u < m ? __shfl(kk, src, TPR) : cur;
-                const T *p = grad + (size_t)__shfl(pp, src, TPR) * gstride + c;
-                if (n == 8) x[u] = load8_raw(p);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[u][e] = e < n ? p[e] : (T)0.f;
+                // one team is the wave: scalar registers and branches
+                const uint32_t kv = TPR == 64 ? __builtin_amdgcn_readlane(kk, src) : __shfl(kk, src, TPR);
+                const uint32_t pv = TPR == 64 ? __builtin_amdgcn_readlane(pp, src) : __shfl(pp, src, TPR);
+                k[u] = g + u < m ? kv : cur;
+                const T *p = grad + (size_t)pv * gstride + c;
+                x[u] = load8_raw_n(p, n);
             }
 #pragma unroll
             for (int u = 0; u < 8; ++u)
@@ -253,7 +278,6 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restri
                         acc = splat8(0.f);
                         cur = k[u];
                         older = false;
-                        start = b + g + u;
                     }
                     acc += widen<T>(x[u]);
                 }
@@ -263,44 +287,38 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restri
     if (cur < V) flush(i1, next == cur);
 }
 
-// Tokens whose rows cross chunk borders: their pieces in chunk order.  Tokens without rows: zeros.  (The rest is written.)
-// Column groups of eight; where they are fewer than the threads, the pieces of a token are shared out and joined in order.
+// Tokens whose rows cross chunk borders: their pieces in chunk order.  A workgroup for each chunk and 256 columns; the one whose chunk
+// holds such a token's first row, but not its last, adds the token's pieces: sixteen shares of consecutive pieces, joined in
+// order.  The workgroups behind them clear the rows of tokens that do not occur, where the sort has not done it.
 template <class T>
-__global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t *__restrict__ begin, const uint32_t *__restrict__ last, int64_t V, int per_block,
-                                                         const float *__restrict__ part, int chunk, int d, float scale, int cols, T *__restrict__ out) {
-    __shared__ float sh[256 * 8];
-    const int cl = threadIdx.x & (cols - 1), share = threadIdx.x / cols, shares = 256 / cols;      // cols: a power of two
-    const int64_t v0 = (int64_t)blockIdx.x * per_block, v1 = v0 + per_block < V ? v0 + per_block : V;
-    __shared__ uint32_t ends[64], starts[64];
-    if (threadIdx.x < v1 - v0) { ends[threadIdx.x] = last[v0 + threadIdx.x]; starts[threadIdx.x] = begin[v0 + threadIdx.x]; }
+__global__ __launch_bounds__(512) void embed_join_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ last, int64_t rows, uint32_t V,
+                                                         const float *__restrict__ part, int chunk, int ntile, int d, float scale, T *__restrict__ out, EmbFill fill) {
+    if ((int64_t)blockIdx.x >= fill.first) { emb_fill(fill); return; }
+    __shared__ __attribute__((aligned(32))) float sh[512 * 8];
+    const int64_t ch = blockIdx.x / ntile, i0 = ch * chunk, i1 = i0 + chunk;
+    if (i1 >= rows) return;
+    const uint32_t cur = key[i1 - 1], after = key[i1], prior = i0 > 0 ? key[i0 - 1] : ~0u;
+    if (cur >= V || after != cur || prior == cur) return;
+    const uint32_t count = (last[cur] - 1) / chunk - (uint32_t)ch + 1, each = (count + 15) / 16;
+    const int cl = threadIdx.x & 31, share = threadIdx.x >> 5, c = ((int)(blockIdx.x - ch * ntile) * 32 + cl) * 8, n = d - c;
+    const uint32_t a = share * each, b = a + each < count ? a + each : count;
+    const float *src = part + (size_t)ch * 2 * d + c;  // piece 0 is the chunk's second one, the others are first ones
+    f8 s = splat8(0.f);
+    if (n >= 8)
+        for (uint32_t k = a; k < b; k += 8) {           // eight at a time, the last ones too (a remainder would wait for each)
+            f8 x[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) { const uint32_t q = k + u < b ? k + u : b - 1; x[u] = load8(src + ((size_t)q * 2 + (q == 0 ? 1 : 0)) * d); }
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) if (k + u < b) s += x[u];
+        }
+    else if (n > 0)
+        for (uint32_t k = a; k < b; ++k) s += load8_n(src + ((size_t)k * 2 + (k == 0 ? 1 : 0)) * d, n);
+    *(f8 *)(sh + threadIdx.x * 8) = s;
     __syncthreads();
-    for (int64_t v = v0; v < v1; ++v) {                // the same for the whole block
-        const uint32_t e = ends[v - v0];
-        T *dst = out + (size_t)v * d;
-        if (e == 0) {
-            for (int c = threadIdx.x * 8; c < d; c += 2048) store8_n(dst + c, splat8(0.f), d - c < 8 ? d - c : 8);
-            continue;
-        }
-        const uint32_t c0 = starts[v - v0] / chunk, c1 = (e - 1) / chunk;
-        if (c0 == c1) continue;
-        const uint32_t count = c1 - c0 + 1, each = (count + shares - 1) / shares;
-        const uint32_t a = share * each, b = a + each < count ? a + each : count;
-        for (int cb = 0; cb < d; cb += cols * 8) {
-            const int c = cb + cl * 8, n = d - c < 8 ? d - c : 8;
-            f8 s = splat8(0.f);
-            if (n > 0)
-#pragma unroll 4
-                for (uint32_t k = a; k < b; ++k) s += load8_n(part + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * d + c, n);
-            if (shares > 1) {
-                __syncthreads();
-                *(f8 *)(sh + threadIdx.x * 8) = s;
-                __syncthreads();
-                if (share == 0)
-                    for (int q = 1; q < shares; ++q) s += *(const f8 *)(sh + (q * cols + cl) * 8);
-            }
-            if (share == 0 && n > 0) store8_n(dst + c, s * scale, n);
-        }
-    }
+    if (share != 0 || n <= 0) return;
+    for (int q = 1; q < 16; ++q) s += *(const f8 *)(sh + (q * 32 + cl) * 8);
+    store8_n(out + (size_t)cur * d + c, s * scale, n);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -311,7 +329,7 @@ struct GradPlan {
     bool few = false, lds = false;
     int64_t per_block = 0;             // few: rows per block; radix sort: list entries per block
     int nblk = 0, chunk = 0, nchunk = 0, passes = 0;
-    size_t part = 0, key[2] = {}, pos[2] = {}, hist = 0, begin = 0, last = 0, bytes = 0;      // offsets into the workspace
+    size_t part = 0, key[2] = {}, pos[2] = {}, hist = 0, last = 0, bytes = 0;      // offsets into the workspace
 };
 
 GradPlan grad_plan(int64_t rows, int64_t V, int64_t d) {
@@ -343,7 +361,6 @@ GradPlan grad_plan(int64_t rows, int64_t V, int64_t d) {
     auto take = [&](size_t n) { const size_t at = o; o += align256(n); return at; };
     for (int k = 0; k < (p.lds ? 1 : 2); ++k) { p.key[k] = take(rows * 4); p.pos[k] = take(rows * 4); }
     p.hist = take(p.lds ? 0 : EMB_MAXB * 256 * 4);
-    p.begin = take(V * 4);
     p.last = take(V * 4);
     p.part = take((size_t)p.nchunk * 2 * d * 4);
     p.bytes = o;
@@ -390,7 +407,7 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
         return 0;
     }
     uint32_t *key[2] = {(uint32_t *)(ws + p.key[0]), (uint32_t *)(ws + p.key[1])}, *pos[2] = {(uint32_t *)(ws + p.pos[0]), (uint32_t *)(ws + p.pos[1])};
-    uint32_t *hist = (uint32_t *)(ws + p.hist), *begin = (uint32_t *)(ws + p.begin), *last = (uint32_t *)(ws + p.last);
+    uint32_t *hist = (uint32_t *)(ws + p.hist), *last = (uint32_t *)(ws + p.last);
     float *part = (float *)(ws + p.part);
     int now = 0;
     if (p.lds) {
@@ -403,12 +420,21 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
         hipLaunchKernelGGL(kern, dim3(1 + zero), dim3(1024), (size_t)n2 * 8, st, id, (int)rows, n2, V, pad, key[0], pos[0], last);
         TOK_TRY(hipGetLastError());
     } else {
+        // The first scatter marks the tokens that occur; from then on 512 workgroups more per launch clear the others' rows
+        // (32768 x 2048 bf16 over 64000 tokens).
+        const int64_t launches = 2 * (p.passes - 1);
         for (int q = 0; q < p.passes; ++q) {
             const I *src = q == 0 ? id : nullptr;
-            hipLaunchKernelGGL((embed_hist_kernel<I>), dim3(p.nblk), dim3(256), 0, st, src, key[now], rows, p.per_block, V, pad, 8 * q, hist, q == 0 ? last : nullptr);
+            EmbFill f[2] = {{last, (uint16_t *)out, 0, 0, d * (int64_t)(sizeof(T) / 2), p.nblk}, {last, (uint16_t *)out, 0, 0, d * (int64_t)(sizeof(T) / 2), p.nblk}};
+            for (int h = 0; h < 2 && q > 0; ++h) {
+                f[h].v0 = V * (2 * (q - 1) + h) / launches;
+                f[h].v1 = V * (2 * (q - 1) + h + 1) / launches;
+            }
+            const unsigned grid = p.nblk + (q > 0 ? 512 : 0);
+            hipLaunchKernelGGL((embed_hist_kernel<I>), dim3(grid), dim3(256), 0, st, src, key[now], rows, p.per_block, V, pad, 8 * q, hist, q == 0 ? last : nullptr, f[0]);
             TOK_TRY(hipGetLastError());
-            hipLaunchKernelGGL((embed_scatter_kernel<I>), dim3(p.nblk), dim3(256), 0, st, src, key[now], q == 0 ? nullptr : pos[now], rows, p.per_block, V, pad, 8 * q,
-                               hist, key[now ^ 1], pos[now ^ 1]);
+            hipLaunchKernelGGL((embed_scatter_kernel<I>), dim3(grid), dim3(256), 0, st, src, key[now], q == 0 ? nullptr : pos[now], rows, p.per_block, V, pad, 8 * q,
+                               hist, key[now ^ 1], pos[now ^ 1], q == 0 && p.passes > 1 ? last : nullptr, f[1]);
             TOK_TRY(hipGetLastError());
             now ^= 1;
         }
@@ -417,12 +443,16 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
     const int64_t ntile = ceil_div(d, (int64_t)tpr * 8), units = p.nchunk * ntile;
     auto sum = tpr == 8 ? embed_sum_kernel<T, 8> : tpr == 16 ? embed_sum_kernel<T, 16> : tpr == 32 ? embed_sum_kernel<T, 32> : embed_sum_kernel<T, 64>;
     hipLaunchKernelGGL(sum, dim3((unsigned)ceil_div(units, 256 / tpr)), dim3(256), 0, st, key[now], pos[now], rows, g, gs, (uint32_t)V, (int)d, scale, p.chunk, (int)ntile,
-                       (T *)out, begin, last, part);
+                       (T *)out, last, part);
     TOK_TRY(hipGetLastError());
-    int per = (int)(V / 1024);
-    per = per < 1 ? 1 : per > 64 ? 64 : per;
-    hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)ceil_div(V, per)), dim3(256), 0, st, begin, last, V, per, part, p.chunk, (int)d, scale,
-                       pow2_at_least(ceil_div(d, 8), 1, 256), (T *)out);
+    // (a chunk's number fits: at least 8 rows each)
+    const int jtile = (int)ceil_div(d, 256);
+    const int64_t joins = p.nchunk * (int64_t)jtile;
+    if (joins > 0x7ff00000ll) return dnag_fail(DNAG_E_ARG, "rows=%lld x dim=%lld: too many pieces for one launch", (long long)rows, (long long)d);
+    const int64_t clear = p.passes > 1 ? 0 : V < 1024 ? V : 1024;
+    const EmbFill f = {last, (uint16_t *)out, 0, V, d * (int64_t)(sizeof(T) / 2), (int)joins};
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)(joins + clear)), dim3(512), 0, st, key[now], last, rows, (uint32_t)V, part, p.chunk, jtile, (int)d, scale,
+                       (T *)out, f);
     TOK_TRY(hipGetLastError());
     return 0;
 }
