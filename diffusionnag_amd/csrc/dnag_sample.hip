@@ -25,7 +25,7 @@
 #include <math.h>
 
 #define SMP_BINS 2048
-#define SMP_RANGE 28.0f          // exp(-28) < 2^-40: weights beyond are 0
+#define SMP_RANGE 29.0f          // 2^40 exp(-29) < 1/2: weights beyond (the last step) are 0
 #define SMP_BITS 40
 #define SMP_MAX_V (1 << 20)      // sums stay below 2^60
 #define SMP_LIST 2048            // logits that are sorted in LDS
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     __shared__ float queue[NW][512];
     __shared__ u64 ws[NW];
     __shared__ float wf[NW];
-    __shared__ int wi[2][3 * NW];
+    __shared__ int wi[2][8 * NW];
     __shared__ u64 found[3];                           // bin, sum before it, sum in it
     __shared__ int at_found, listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -162,29 +162,27 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     const int V = a.V;
     const RowSet s = row_set(a, row);
     // f(first index, eight logits as they are), called by whole waves: a lane past the end has -inf, and the row's last piece
-    // that is shorter than eight comes as the row's last eight with what was seen before set to -inf.  Four loads are under way before the
-    // first is used (one at a time, a pass over 128000 logits took as long as sixteen trips to the cache).
+    // that is shorter than eight comes as the row's last eight with what was seen before set to -inf.  A rolled loop with three
+    // pieces under way ahead of the one that is worked on: a workgroup runs through each pass once, so what counts is the code's size (with
+    // the pieces unrolled the passes waited for instructions: 256 rows of 128000 with top-p 114 us, rolled 67).
     auto each8 = [&](auto f) {
         typedef typename Vec8<T>::type raw8;
-        constexpr int U = 4, STEP = NTHR * 8;
-        for (int c0 = 0; c0 < V; c0 += U * STEP) {
-            raw8 r[U];
+        constexpr int STEP = NTHR * 8;
+        auto ask = [&](int c) { return load8_raw(l + (c + 8 <= V ? c : V - 8)); };
+        int c = tid * 8;
+        raw8 r0 = ask(c), r1 = ask(c + STEP), r2 = ask(c + 2 * STEP);
+#pragma unroll 1
+        for (; __builtin_amdgcn_readfirstlane(c) < V; c += STEP) {
+            const raw8 now = r0;
+            r0 = r1;
+            r1 = r2;
+            r2 = ask(c + 3 * STEP);
+            f8 v = widen<T>(now);
+            if (c + 8 > V) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int c = c0 + u * STEP + tid * 8;
-                if (c < V) r[u] = load8_raw(l + (c + 8 <= V ? c : V - 8));
+                for (int e = 0; e < 8; ++e) if (e < 8 - (V - c)) v[e] = -INFINITY;
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int c = c0 + u * STEP + tid * 8;
-                if (__builtin_amdgcn_readfirstlane(c) >= V) break;
-                f8 v = widen<T>(r[u]);
-                if (c + 8 > V) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) if (e < 8 - (V - c)) v[e] = -INFINITY;
-                }
-                f(c + 8 <= V ? c : V - 8, v);
-            }
+            f(c + 8 <= V ? c : V - 8, v);
         }
     };
     float mine = -INFINITY;                            // this lane's largest logit (the maximum passes NaN over)
@@ -238,6 +236,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             const u64 x = tid < n ? hist[tid] : 0;
             int r = 0;
             if (tid < n)
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) { const u64 y = hist[j]; r += y > x || (y == x && j < tid); }
             __syncthreads();
             if (tid < n) hist[r] = x;
@@ -281,18 +280,40 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     };
     // ---- top-k on a short list ---------------------------------------------------------------------------------------
     if (s.k > 0 && s.k <= NTHR && s.k < V) {
-        // upper bits of the k-th largest of the lanes' maxima, two bits at a time: rounding it down keeps a lower bound
-        const uint32_t key = ordered(mine);
+        // A bound that k of the lanes' maxima reach, and not many more: the ordered bits of the maximum less a power of two (2^23 is an
+        // octave), eight powers at a time; then, if that leaves too many, the k-th largest's upper bits, two at a time.
+        const uint32_t key = ordered(mine), top_key = ordered(m);
         uint32_t low = 0;
-        for (int b = 30; b >= 12; b -= 2) {
-            int *buf = wi[(b >> 1) & 1];
-            const int c1 = __popcll(__ballot(key >= (low | 1u << b))), c2 = __popcll(__ballot(key >= (low | 2u << b))), c3 = __popcll(__ballot(key >= (low | 3u << b)));
-            if (lane == 0) { buf[wave] = c1; buf[NW + wave] = c2; buf[2 * NW + wave] = c3; }
-            __syncthreads();
-            int n1 = 0, n2 = 0, n3 = 0;
+        int reach = 0;
+        for (int b = 18; b < 32 && reach < s.k; b += 8) {
+            int *buf = wi[(b >> 3) & 1];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { n1 += buf[w]; n2 += buf[NW + w]; n3 += buf[2 * NW + w]; }
-            low |= (n3 >= s.k ? 3u : n2 >= s.k ? 2u : n1 >= s.k ? 1u : 0u) << b;
+            for (int q = 0; q < 8; ++q) {
+                const uint32_t want = b + q < 32 && top_key > 1u << (b + q) ? top_key - (1u << (b + q)) : 0;
+                const int c = __popcll(__ballot(key >= want));
+                if (lane == 0) buf[q * NW + wave] = c;
+            }
+            __syncthreads();
+            for (int q = 0; q < 8 && reach < s.k; ++q) {
+                reach = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) reach += buf[q * NW + w];
+                low = b + q < 32 && top_key > 1u << (b + q) ? top_key - (1u << (b + q)) : 0;
+            }
+        }
+        if (reach > 2 * s.k + 256) {
+            low = 0;
+            __syncthreads();
+            for (int b = 30; b >= 12; b -= 2) {
+                int *buf = wi[(b >> 1) & 1];
+                const int c1 = __popcll(__ballot(key >= (low | 1u << b))), c2 = __popcll(__ballot(key >= (low | 2u << b))), c3 = __popcll(__ballot(key >= (low | 3u << b)));
+                if (lane == 0) { buf[wave] = c1; buf[NW + wave] = c2; buf[2 * NW + wave] = c3; }
+                __syncthreads();
+                int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) { n1 += buf[w]; n2 += buf[NW + w]; n3 += buf[2 * NW + w]; }
+                low |= (n3 >= s.k ? 3u : n2 >= s.k ? 2u : n1 >= s.k ? 1u : 0u) << b;
+            }
         }
         // as a logit (what lies between -0 and +0 becomes 0, a key below every logit's becomes -inf)
         float from = low <= 0x007fffffu ? -INFINITY : value_of((u64)low << 32);
@@ -342,12 +363,8 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         }
     }
     // ---- any cut -----------------------------------------------------------------------------------------------------
-    const float per_step = (float)(s.c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE));
-    auto step_of = [&](float x) -> int {               // never falls as x falls
-        if (x == m) return 0;
-        const float q = (m - x) * per_step;
-        return q < (float)(SMP_BINS - 1) ? (int)q : SMP_BINS - 1;
-    };
+    const float per_step = fminf((float)(s.c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE)), 1e30f);
+    auto step_of = [&](float x) { return inf ? (x == m ? 0.f : SMP_BINS - 1.f) : fminf((m - x) * per_step, SMP_BINS - 1.f); };      // never falls as x falls; the step is its whole part
     auto inside = [&](const Cut &c, float x, int i) { return x > c.x || (x == c.x && i <= c.at); };
     auto clear = [&]() {
         __syncthreads();
@@ -372,15 +389,16 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         return want;
     };
     // cut where the sum of wt over the elements that `was` keeps reaches its goal
-    auto find_cut = [&](const Cut &was, auto wt, auto goal) {
+    auto find_cut = [&](const Cut &was, bool counts, auto wt, auto goal) {
+        const bool any = was.x == -INFINITY;
         clear();
         each8([&](int i0, const f8 &v) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (inside(was, v[e], i0 + e)) {
-                    const u64 w = wt(v[e]);
-                    if (w) atomicAdd(&hist[step_of(v[e])], w);
-                }
+            for (int e = 0; e < 8; ++e) {
+                const float q = step_of(v[e]);
+                const u64 w = wt(v[e]);
+                if ((counts ? v[e] > -INFINITY : q < SMP_BINS - 1.f) && (any || inside(was, v[e], i0 + e))) atomicAdd(&hist[(int)q], w);
+            }
         });
         u64 want = scan(goal);
         if (found[0] == SMP_BINS) return was;          // the goal is not reached: all are kept
@@ -389,7 +407,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         // bounds of the step, a little wide, spare most logits the exact test
         const float wide = (float)step / per_step, far = (float)(step + 1) / per_step, slack = (fabsf(m) + far) * 1e-6f;
         const float to = m - wide + slack, from = step == SMP_BINS - 1 ? -INFINITY : m - far - slack;
-        const int n = collect(from == from ? from : -INFINITY, to == to ? to : INFINITY, [&](float x, int i) { return inside(was, x, i) && step_of(x) == step; });
+        const int n = collect(from == from ? from : -INFINITY, to == to ? to : INFINITY, [&](float x, int i) { return inside(was, x, i) && (int)step_of(x) == step; });
         if (n <= SMP_LIST) {                           // the first of the sorted ones whose running sum reaches what is left
             sort_falling(n);
             constexpr int EACH = SMP_LIST / NTHR;
@@ -414,7 +432,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             each8([&](int i0, const f8 &v) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (inside(was, v[e], i0 + e) && step_of(v[e]) == step) {
+                    if (inside(was, v[e], i0 + e) && (int)step_of(v[e]) == step) {
                         const uint32_t k = ordered(clean(v[e]));
                         if (shift == 21 || (k >> (shift + bits)) == prefix)
                             atomicAdd(&hist[(1 << bits) - 1 - ((k >> shift) & ((1u << bits) - 1))], wt(v[e]));
@@ -451,8 +469,8 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         return c;
     };
     Cut cut{-INFINITY, -1};                            // everything that can be drawn
-    if (s.k > 0 && s.k < V) cut = find_cut(cut, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
-    if (s.p < 1.0) cut = find_cut(cut, weight, [&](u64 total) { return goal_of(s.p, total); });
+    if (s.k > 0 && s.k < V) cut = find_cut(cut, true, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
+    if (s.p < 1.0) cut = find_cut(cut, false, weight, [&](u64 total) { return goal_of(s.p, total); });
     // min-p is a cut too: the smallest logit that weighs enough, by halving the ordered bit patterns up to the maximum's
     if (s.minw > 0.0) {
         uint32_t lo = 0x007fffffu, hi = ordered(m);    // lo: -inf, too light; hi: weighs enough, or is the largest anyway
@@ -500,7 +518,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             for (int e = 0; e < 8; ++e) {
                 const bool in = inside(cut, v[e], i0 + e);
                 const uint64_t b = __ballot(in);
-                if (in) q[n + __popcll(b & ((1ull << lane) - 1))] = v[e];
+                if (in) q[__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, n))] = v[e];
                 n += __popcll(b);
             }
             wave_fence();
