@@ -134,6 +134,29 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
 #pragma unroll
         for (int k = 0; k < NA; ++k) acc[k][j] = splat8(0.f);
     }
+    // A lane's share of the weights and of the gate row, fp32, in LDS that only it reads (no barriers): the row body uses them five
+    // times, and every one of those would be a trip to L2.
+    constexpr bool HELD = NV == 1;
+    extern __shared__ __attribute__((aligned(16))) float held[];       // [3][2][threads][4]: post weight, pre weight, gate
+    const int threads = blockDim.x;
+    auto hold = [&](int k, const f8 &v) {
+        *(float4 *)(held + (size_t)((2 * k) * threads + threadIdx.x) * 4) = float4{v[0], v[1], v[2], v[3]};
+        *(float4 *)(held + (size_t)((2 * k + 1) * threads + threadIdx.x) * 4) = float4{v[4], v[5], v[6], v[7]};
+    };
+    auto held_at = [&](int k) {
+        const float4 p = *(const float4 *)(held + (size_t)((2 * k) * threads + threadIdx.x) * 4), q = *(const float4 *)(held + (size_t)((2 * k + 1) * threads + threadIdx.x) * 4);
+        return f8{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    };
+    auto small = [&](const void *p, int bit, size_t at, int j, float none) {
+        return p && n[j] > 0 ? load8_either<TY>(p, a.small32 & bit, at, n[j]) : splat8(none);
+    };
+    if constexpr (HELD) {
+        hold(0, small(a.pw, 2, lane * 8, 0, 1.f));
+        hold(1, small(a.qw, 4, lane * 8, 0, 1.f));
+    }
+    auto post_weight = [&](int j) { if constexpr (HELD) return held_at(0); else return small(a.pw, 2, (j * TPR + lane) * 8, j, 1.f); };
+    auto pre_weight = [&](int j) { if constexpr (HELD) return held_at(1); else return small(a.qw, 4, (j * TPR + lane) * 8, j, 1.f); };
+    auto gate_of = [&](int j, size_t g0) { if constexpr (HELD) return held_at(2); else return small(a.gate, 1, g0 + (j * TPR + lane) * 8, j, 1.f); };
     auto one_row = [&](int64_t row, size_t g0) __attribute__((always_inline)) {      // as a call its sums would live in memory
         f8 x[NV], y[NV], gx[NV], gh[NV];
         typename Vec8<TX>::type rx[NV], rgx[NV];
@@ -155,18 +178,15 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
             gx[j] = n[j] > 0 && a.gx ? widen<TX>(rgx[j]) : splat8(0.f);
             gh[j] = n[j] > 0 && a.gh ? widen<TY>(rgh[j]) : splat8(0.f);
         }
-        auto small = [&](const void *p, int bit, size_t at, int j, float none) {
-            return p && n[j] > 0 ? load8_either<TY>(p, a.small32 & bit, at, n[j]) : splat8(none);
-        };
         float ry = 0.f;
         if (a.y) {
             ry = normalise<LN>(y, n, sum, a.eps, a.inv_d);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * TPR + lane) * 8;
-                f8 v = y[j] * small(a.pw, 2, c, j, 1.f);
+                f8 v = y[j] * post_weight(j);
                 if (LN) v += small(a.pb, 2, c, j, 0.f);
-                x[j] = x[j] * a.rs + v * small(a.gate, 1, g0 + c, j, 1.f);
+                x[j] = x[j] * a.rs + v * gate_of(j, g0);
             }
         }
         if (a.pre) {
@@ -176,7 +196,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
             for (int j = 0; j < NV; ++j) {
                 acc[0][j] += gh[j] * x[j];
                 if constexpr (LN) acc[2][j] += gh[j];
-                gh[j] *= small(a.qw, 4, (j * TPR + lane) * 8, j, 1.f);
+                gh[j] *= pre_weight(j);
                 s1 += sum8(gh[j] * x[j]);
                 if (LN) s2 += sum8(gh[j]);
             }
@@ -194,11 +214,11 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * TPR + lane) * 8;
-            const f8 w = small(a.pw, 2, c, j, 1.f);
+            const f8 w = post_weight(j);
             f8 v = y[j] * w;
             if (LN) v += small(a.pb, 2, c, j, 0.f);
             dg[j] += gx[j] * v;
-            gx[j] *= small(a.gate, 1, g0 + c, j, 1.f);
+            gx[j] *= gate_of(j, g0);
             if (n[j] < 8)                              // columns past d carry the LayerNorm means of gx: nothing of them is summed
 #pragma unroll
                 for (int e = 0; e < 8; ++e) if (e >= n[j]) gx[j][e] = 0.f;
@@ -259,6 +279,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel
         const int s = few ? 0 : (int)(w - g * a.S);
         const int64_t end = (g + 1) * a.rpg, r0 = g * a.rpg + s * a.split_rows, r1 = few || r0 + a.split_rows > end ? end : r0 + a.split_rows;
         clear();
+        if constexpr (HELD) if (g < a.G) hold(2, small(a.gate, 1, (size_t)g * a.d + lane * 8, 0, 1.f));
         if (g < a.G)
             for (int64_t r = r0 + sub; r < r1; r += few ? a.cell : NT) one_row(r, (size_t)g * a.d);
         if (!a.dgate) continue;
@@ -325,10 +346,6 @@ int lanes_for(int64_t d) {                             // lanes of a team: eight
     const int64_t v = ceil_div(d, 8);
     return v <= 8 ? 8 : v <= 32 ? 32 : pow2_at_least(v, 64, 1024);
 }
-#ifndef BNG
-#define BNG 256
-#endif
-int grad_lanes_for(int64_t d) { return d > 1024 && d <= 2048 ? BNG : lanes_for(d); }
 struct BnPlan {
     int tpr, nt, nblk, S, na, cell;
     int64_t split;
@@ -336,15 +353,12 @@ struct BnPlan {
 };
 BnPlan grad_plan(const dnag_block_norms_args &p) {
     BnPlan q;
-    q.tpr = grad_lanes_for(p.dim);
+    q.tpr = lanes_for(p.dim);
     q.nt = q.tpr <= 64 ? 256 / q.tpr : 1;
     q.na = p.layer_norm ? 4 : 2;
     const int64_t G = p.gate_rows, rpg = p.rows / G;
     // two blocks of 256 lanes for every CU: fewer partial sums than a block per row, and enough rows in flight
-#ifndef BNT
-#define BNT 1024
-#endif
-    const int64_t target = q.tpr <= 64 ? 512 : q.tpr <= 256 ? BNT : q.tpr == 512 ? 512 : 256;
+    const int64_t target = q.tpr <= 64 ? 512 : q.tpr <= 256 ? 1024 : q.tpr == 512 ? 512 : 256;
     q.S = 1;
     if (rpg >= q.nt) {
         int64_t s = ceil_div(target, G), most = ceil_div(rpg, q.nt);
@@ -386,35 +400,34 @@ BnArgs common_args(const dnag_block_norms_args &p) {
     return a;
 }
 template <class TX, class TY, int TPR, int NV, bool LN>
-void launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
-    if (grad) hipLaunchKernelGGL((block_norms_grad_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(TPR <= 64 ? 256 : TPR), 0, st, a);
-    else hipLaunchKernelGGL((block_norms_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(TPR <= 64 ? 256 : TPR), 0, st, a);
+int launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
+    constexpr int threads = TPR <= 64 ? 256 : TPR;
+    if (grad) {
+        const size_t lds = NV == 1 ? (size_t)3 * threads * 32 : 0;
+        static LdsLimit limit;
+        if (int rc = limit.allow((const void *)block_norms_grad_kernel<TX, TY, TPR, NV, LN>, lds)) return rc;
+        hipLaunchKernelGGL((block_norms_grad_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(threads), lds, st, a);
+    } else hipLaunchKernelGGL((block_norms_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(threads), 0, st, a);
+    return 0;
 }
 template <class TX, class TY, bool LN>
-void launch_width(const BnArgs &a, int tpr, bool grad, unsigned blocks, hipStream_t st) {
+int launch_width(const BnArgs &a, int tpr, bool grad, unsigned blocks, hipStream_t st) {
     switch (tpr) {
-        case 8: launch<TX, TY, 8, 1, LN>(a, grad, blocks, st); break;
-        case 32: launch<TX, TY, 32, 1, LN>(a, grad, blocks, st); break;
-        case 64:
-            if (a.d > 512) launch<TX, TY, 64, 4, LN>(a, grad, blocks, st);
-            else launch<TX, TY, 64, 1, LN>(a, grad, blocks, st);
-            break;
-        case 128:
-            if (a.d > 1024) launch<TX, TY, 128, 2, LN>(a, grad, blocks, st);
-            else launch<TX, TY, 128, 1, LN>(a, grad, blocks, st);
-            break;
-        case 256: launch<TX, TY, 256, 1, LN>(a, grad, blocks, st); break;
-        case 512: launch<TX, TY, 512, 1, LN>(a, grad, blocks, st); break;
+        case 8: return launch<TX, TY, 8, 1, LN>(a, grad, blocks, st);
+        case 32: return launch<TX, TY, 32, 1, LN>(a, grad, blocks, st);
+        case 64: return launch<TX, TY, 64, 1, LN>(a, grad, blocks, st);
+        case 128: return launch<TX, TY, 128, 1, LN>(a, grad, blocks, st);
+        case 256: return launch<TX, TY, 256, 1, LN>(a, grad, blocks, st);
+        case 512: return launch<TX, TY, 512, 1, LN>(a, grad, blocks, st);
         default:
-            if (a.d <= 8192) launch<TX, TY, 1024, 1, LN>(a, grad, blocks, st);
-            else launch<TX, TY, 1024, 2, LN>(a, grad, blocks, st);
+            if (a.d <= 8192) return launch<TX, TY, 1024, 1, LN>(a, grad, blocks, st);
+            return launch<TX, TY, 1024, 2, LN>(a, grad, blocks, st);
     }
 }
 template <class TX, class TY>
 int launch_types(const dnag_block_norms_args &p, const BnArgs &a, int tpr, bool grad, unsigned blocks) {
     hipStream_t st = (hipStream_t)p.stream;
-    if (p.layer_norm) launch_width<TX, TY, true>(a, tpr, grad, blocks, st);
-    else launch_width<TX, TY, false>(a, tpr, grad, blocks, st);
+    if (int rc = p.layer_norm ? launch_width<TX, TY, true>(a, tpr, grad, blocks, st) : launch_width<TX, TY, false>(a, tpr, grad, blocks, st)) return rc;
     TOK_TRY(hipGetLastError());
     return 0;
 }

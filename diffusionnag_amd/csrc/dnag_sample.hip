@@ -147,6 +147,7 @@ struct Cut { float x; int at; };   // kept: larger logits, and equal ones up to 
 template <class T, int NTHR>
 __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     constexpr int NW = NTHR / 64, PER = SMP_BINS / NTHR;
+    constexpr bool COUNTED = __is_same(T, tbf16);
     extern __shared__ u64 piece[];                     // sums of 512 logits each, for the draw
     __shared__ u64 hist[SMP_BINS];                     // histogram, or the list of logits that is sorted
     static_assert(SMP_LIST <= SMP_BINS, "the list shares the histogram's memory");
@@ -185,31 +186,10 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             f(c + 8 <= V ? c : V - 8, v);
         }
     };
-    float mine = -INFINITY;                            // this lane's largest logit (the maximum passes NaN over)
-    each8([&](int, const f8 &v) { mine = fmaxf(mine, max8(v)); });
-    mine = clean(mine);
-    float m = team_max<64>(mine);
-    if (lane == 0) wf[wave] = m;
-    if (tid == 0) { at_found = 0x7fffffff; listed = 0; }
-    __syncthreads();
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, wf[w]);
-    if (m == -INFINITY) { if (tid == 0) a.out[row] = -1; return; }
-    if (s.greedy) {
-        if (mine == m) {
-            int first = 0x7fffffff;
-            each8([&](int c, const f8 &v) {
-#pragma unroll
-                for (int e = 7; e >= 0; --e) if (v[e] == m && c + e < first) first = c + e;
-            });
-            atomicMin(&at_found, first);
-        }
-        __syncthreads();
-        if (tid == 0) a.out[row] = at_found;
-        return;
-    }
+    float m = -INFINITY;                               // the row's largest logit
+    double md = 0.0;
+    bool inf = false;
     // an infinite maximum leaves its equals alone: they weigh 1, everything else is below any cut
-    const bool inf = m == INFINITY;
-    const double md = inf ? 0.0 : (double)m;
     auto weight_raw = [&](float x) { return raw_weight(inf ? (x == m ? 0.f : -INFINITY) : x, md, s.c); };
     auto weight = [&](float x) -> u64 { return whole_weight(weight_raw(x)); };
     auto wave_scan = [&](u64 v) {                      // inclusive
@@ -278,8 +258,220 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         __syncthreads();
         return listed;
     };
+    Cut cut{-INFINITY, -1};                            // everything that can be drawn
+    // top-k on a short list, below (a longer list's sorting costs more than counting bf16 values: k = 1000 of 128000, 86 and 52 us)
+    const bool short_list = s.k > 0 && s.k < V && s.k <= (COUNTED && NTHR == 1024 ? 256 : NTHR);
+    bool done = false;                                 // `cut` is final and `piece` holds the kept weights' sums
+    const int pieces = (V + 511) / 512;
+    auto inside = [&](const Cut &c, float x, int i) { return x > c.x || (x == c.x && i <= c.at); };
+    // ---- bf16: few values, counted ---------------------------------------------------------------------------------------
+    // A row of bf16 logits holds few different values.  Those of magnitude 2^-9 .. 2^9 are counted (4608 slots in falling order), the
+    // exponentials, sums and cuts are taken over the slots, and the draw looks its weights up.  What is nearer to 0 (slot HALF)
+    // is listed and weighed one by one.  Rows that do not fit -- a logit from 512 on, a list that is too short, a cut between the
+    // listed ones -- go the general way.  256 rows of 128000, top-p: 110 us the general way, 46 this way.
+    if constexpr (sizeof(T) == 2 && NTHR == 1024 && COUNTED) {
+        constexpr int HALF = 18 * 128, EACH = 5, SLOTS = EACH * NTHR;
+        static_assert(2 * HALF + 1 <= SLOTS && sizeof(uint32_t) * SLOTS <= sizeof(queue), "slots");
+        uint32_t *count = (uint32_t *)&queue[0][0];
+        u64 *table = piece + pieces;
+        float *near = (float *)hist;                   // [SMP_LIST], then [SMP_LIST] indices of equal logits at the cut
+        int *ties = (int *)(near + SMP_LIST);
+        auto slot_of = [&](float x) {
+            const uint32_t h = __float_as_uint(x) >> 16, i = (h & 0x7fffu) - 0x3b00u;
+            return i < (uint32_t)HALF ? (int)(h & 0x8000u ? HALF + 1 + i : HALF - 1 - i) : -1;
+        };
+        auto value_at = [&](int r) { return __uint_as_float((r < HALF ? 0x3b00u + (HALF - 1 - r) : 0xbb00u + (r - HALF - 1)) << 16); };
+        if (!s.greedy && (s.p < 1.0 || (s.k > 0 && s.k < V)) && !short_list) {
+            for (int r = tid; r < SLOTS; r += NTHR) count[r] = 0;
+            if (tid == 0) { listed = 0; at_found = 0; found[0] = SLOTS; found[1] = SLOTS; found[2] = 0; }
+            __syncthreads();
+            int odd = 0;                               // 1: a logit below -512, 2: one from 512 on
+            each8([&](int, const f8 &v) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int r = slot_of(v[e]);
+                    if (r >= 0) atomicAdd(&count[r], 1u);
+                    else if (fabsf(v[e]) < 1.0f) {
+                        const int at = atomicAdd(&listed, 1);
+                        if (at < SMP_LIST) near[at] = clean(v[e]);
+                    } else if (v[e] > -INFINITY) odd |= v[e] > 0.f ? 2 : 1;
+                }
+            });
+            if (odd) atomicOr(&at_found, odd);
+            __syncthreads();
+            const int n_near = listed;
+            bool fits = n_near <= SMP_LIST && !(at_found & 2);
+            // the maximum: the first slot that is not empty, or among the listed ones
+            uint32_t cnt[EACH];
+            int first = SLOTS;
+#pragma unroll
+            for (int q = EACH - 1; q >= 0; --q) {
+                const int r = tid * EACH + q;
+                cnt[q] = r == HALF ? (uint32_t)n_near : count[r];
+                if (cnt[q] && r != HALF) first = r;
+            }
+            float top = first < SLOTS ? value_at(first) : -INFINITY;
+            if (fits) for (int i = tid; i < n_near; i += NTHR) top = fmaxf(top, near[i]);
+            top = team_max<64>(top);
+            if (lane == 0) wf[wave] = top;
+            __syncthreads();
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, wf[w]);
+            // logits below -512 may be left out where they weigh nothing
+            fits = fits && top > -INFINITY && (!(at_found & 1) || ((double)top + 512.0) * s.c > 42.0) && !(s.minw > 1099511627776.0);
+            if (fits) {
+                m = top;
+                md = (double)m;
+                u64 w[EACH], sum = 0, total, near_sum;
+                bool light[EACH];                      // min-p drops the slot
+                u64 near_mine = 0;
+                int heavy = 0;
+                for (int i = tid; i < n_near; i += NTHR) { const double v = weight_raw(near[i]); near_mine += whole_weight(v); heavy += v >= s.minw; }
+                block_before(near_mine, near_sum);
+                u64 heavies;
+                block_before(heavy, heavies);
+#pragma unroll
+                for (int q = 0; q < EACH; ++q) {
+                    const int r = tid * EACH + q;
+                    const double v = cnt[q] && r != HALF ? weight_raw(value_at(r)) : 0.0;
+                    w[q] = whole_weight(v);
+                    light[q] = cnt[q] && (r == HALF ? heavies == 0 : !(v >= s.minw));
+                    table[r] = w[q];
+                }
+                bool mixed = n_near > 0 && heavies > 0 && heavies < (u64)n_near;      // a cut between the listed ones
+                int c_slot = SLOTS, c_ties = 0;        // kept: slots before c_slot, and c_ties logits of it
+                if (s.k > 0 && s.k < V) {
+                    u64 n = 0, all;
+#pragma unroll
+                    for (int q = 0; q < EACH; ++q) n += cnt[q];
+                    u64 before = block_before(n, all);
+#pragma unroll
+                    for (int q = 0; q < EACH; ++q) {
+                        if (before < (u64)s.k && before + cnt[q] >= (u64)s.k) { found[0] = tid * EACH + q; found[2] = s.k - before; }
+                        before += cnt[q];
+                    }
+                    __syncthreads();
+                    c_slot = (int)found[0];
+                    c_ties = c_slot < SLOTS ? (int)found[2] : 0;
+                    mixed = mixed || (c_slot == HALF && c_ties < n_near);
+                    __syncthreads();
+                }
+                if (s.p < 1.0) {
+                    u64 part[EACH];
+#pragma unroll
+                    for (int q = 0; q < EACH; ++q) {
+                        const int r = tid * EACH + q;
+                        const u64 n = r < c_slot ? cnt[q] : r == c_slot ? (u64)c_ties : 0;
+                        part[q] = r == HALF ? (n ? near_sum : 0) : n * w[q];
+                        sum += part[q];
+                    }
+                    u64 before = block_before(sum, total);
+                    const u64 goal = goal_of(s.p, total);
+#pragma unroll
+                    for (int q = 0; q < EACH; ++q) {
+                        if (before < goal && before + part[q] >= goal) {
+                            const int r = tid * EACH + q;
+                            found[1] = r;
+                            found[2] = r == HALF ? (before + part[q] == goal ? (u64)n_near : 0) : (goal - before + w[q] - 1) / w[q];
+                        }
+                        before += part[q];
+                    }
+                    __syncthreads();
+                    c_slot = (int)found[1];            // top-p keeps a part of what top-k kept: its cut is the earlier one
+                    c_ties = (int)found[2];
+                    mixed = mixed || (c_slot == HALF && c_ties == 0);
+                    __syncthreads();
+                }
+                if (s.minw > 0.0) {
+                    if (tid == 0) found[0] = SLOTS;
+                    __syncthreads();
+                    int lightest = SLOTS;
+#pragma unroll
+                    for (int q = EACH - 1; q >= 0; --q) if (light[q]) lightest = tid * EACH + q;
+                    for (int o = 32; o > 0; o >>= 1) { const int b = __shfl_xor(lightest, o, 64); lightest = b < lightest ? b : lightest; }
+                    if (lane == 0) atomicMin(&found[0], (u64)lightest);
+                    __syncthreads();
+                    if ((int)found[0] <= c_slot) { c_slot = (int)found[0]; c_ties = 0; }
+                    __syncthreads();
+                }
+                if (!mixed) {
+                    // equal logits at the cut of which only some are kept are listed by the draw's pass
+                    const bool near_kept = HALF < c_slot || (HALF == c_slot && c_ties > 0);
+                    const int c_count = c_slot < SLOTS && c_slot != HALF ? (int)count[c_slot] : 0;
+                    const bool some = c_slot < SLOTS && c_slot != HALF && c_ties > 0 && c_ties < c_count;
+                    const u64 c_weight = c_slot < SLOTS ? table[c_slot] : 0;
+                    __syncthreads();
+                    for (int r = c_slot + (c_ties > 0 && !some ? 1 : 0) + tid; r < SLOTS; r += NTHR) table[r] = 0;
+                    for (int q = tid; q < pieces; q += NTHR) piece[q] = 0;
+                    if (tid == 0) { listed = 0; at_found = -1; }
+                    __syncthreads();
+                    each8([&](int i0, const f8 &v) {
+                        u64 sum = 0;
+                        uint32_t hit = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int r = slot_of(v[e]);
+                            if (r >= 0) sum += table[r];
+                            else if (near_kept && fabsf(v[e]) < 1.0f) sum += weight(v[e]);
+                            hit |= (r == c_slot ? 1u : 0u) << e;
+                        }
+                        if (some)
+                            for (; hit; hit &= hit - 1) {
+                                const int at = atomicAdd(&listed, 1);
+                                if (at < SMP_LIST) ties[at] = i0 + __ffs(hit) - 1;
+                            }
+                        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+                        if (lane == 0) piece[(i0 + 7) >> 9] = sum;
+                    });
+                    __syncthreads();
+                    const int n = listed;
+                    if (n <= SMP_LIST) {
+                        for (int i = tid; i < n; i += NTHR) {          // those of the lowest indices
+                            const int mine_at = ties[i];
+                            int rank = 0;
+#pragma unroll 8
+                            for (int j = 0; j < n; ++j) rank += ties[j] < mine_at;
+                            if (rank < c_ties) atomicAdd(&piece[mine_at >> 9], c_weight);
+                            if (rank == c_ties - 1) at_found = mine_at;
+                        }
+                        __syncthreads();
+                        if (c_slot == HALF) cut = near_kept ? Cut{-0.001953125f, -1} : Cut{0.001953125f, 0x7fffffff};
+                        else if (c_slot < SLOTS) cut = Cut{value_at(c_slot), some ? at_found : c_ties > 0 ? 0x7fffffff : -1};
+                        done = true;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+    float mine = -INFINITY;                            // this lane's largest logit (the maximum passes NaN over)
+    if (!done) {
+        each8([&](int, const f8 &v) { mine = fmaxf(mine, max8(v)); });
+        mine = clean(mine);
+        m = team_max<64>(mine);
+        __syncthreads();
+        if (lane == 0) wf[wave] = m;
+        if (tid == 0) { at_found = 0x7fffffff; listed = 0; }
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, wf[w]);
+        if (m == -INFINITY) { if (tid == 0) a.out[row] = -1; return; }
+        if (s.greedy) {
+            if (mine == m) {
+                int first = 0x7fffffff;
+                each8([&](int c, const f8 &v) {
+#pragma unroll
+                    for (int e = 7; e >= 0; --e) if (v[e] == m && c + e < first) first = c + e;
+                });
+                atomicMin(&at_found, first);
+            }
+            __syncthreads();
+            if (tid == 0) a.out[row] = at_found;
+            return;
+        }
+        inf = m == INFINITY;
+        md = inf ? 0.0 : (double)m;
+    }
     // ---- top-k on a short list ---------------------------------------------------------------------------------------
-    if (s.k > 0 && s.k <= NTHR && s.k < V) {
+    if (!done && short_list) {
         // A bound that k of the lanes' maxima reach, and not many more: the ordered bits of the maximum less a power of two (2^23 is an
         // octave), eight powers at a time; then, if that leaves too many, the k-th largest's upper bits, two at a time.
         const uint32_t key = ordered(mine), top_key = ordered(m);
@@ -365,7 +557,6 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // ---- any cut -----------------------------------------------------------------------------------------------------
     const float per_step = fminf((float)(s.c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE)), 1e30f);
     auto step_of = [&](float x) { return inf ? (x == m ? 0.f : SMP_BINS - 1.f) : fminf((m - x) * per_step, SMP_BINS - 1.f); };      // never falls as x falls; the step is its whole part
-    auto inside = [&](const Cut &c, float x, int i) { return x > c.x || (x == c.x && i <= c.at); };
     auto clear = [&]() {
         __syncthreads();
         for (int b = tid; b < SMP_BINS; b += NTHR) hist[b] = 0;
@@ -468,7 +659,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         __syncthreads();
         return c;
     };
-    Cut cut{-INFINITY, -1};                            // everything that can be drawn
+    if (!done) {
     if (s.k > 0 && s.k < V) cut = find_cut(cut, true, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
     if (s.p < 1.0) cut = find_cut(cut, false, weight, [&](u64 total) { return goal_of(s.p, total); });
     // min-p is a cut too: the smallest logit that weighs enough, by halving the ordered bit patterns up to the maximum's
@@ -500,8 +691,6 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         if (x > cut.x) cut = Cut{x, at};
         else if (x == cut.x && at < cut.at) cut.at = at;
     }
-    auto kept_weight = [&](float x, int i) -> u64 { return weight(inside(cut, x, i) ? x : -INFINITY); };
-    const int pieces = (V + 511) / 512;
     __syncthreads();
     // A wave's logits of one step of a pass lie in one piece.  Behind a cut few of them are kept: those are moved together in LDS, so that
     // 64 lanes weigh 64 kept logits.
@@ -529,7 +718,9 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         if (lane == 0) piece[(i0 + 7) >> 9] = sum;
     });
     __syncthreads();
+    }
     if (wave != 0) return;
+    auto kept_weight = [&](float x, int i) -> u64 { return weight(inside(cut, x, i) ? x : -INFINITY); };
     u64 total = 0;
     for (int q = lane; q < pieces; q += 64) total += piece[q];
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
@@ -576,7 +767,10 @@ int launch(const SampleArgs &a, hipStream_t st) {
     } else if (a.V <= 4096) {
         hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), (size_t)ceil_div(a.V, 512) * 8, st, a);
     } else {
-        hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), (size_t)ceil_div(a.V, 512) * 8, st, a);
+        const size_t bytes = (size_t)ceil_div(a.V, 512) * 8 + (__is_same(T, tbf16) ? 5120 * 8 : 0);      // pieces, and the slots' weights
+        static LdsLimit limit;
+        if (int rc = limit.allow((const void *)sample_row_kernel<T, 1024>, bytes + 65536)) return rc;      // beside 50 KB that are static
+        hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), bytes, st, a);
     }
     TOK_TRY(hipGetLastError());
     return 0;

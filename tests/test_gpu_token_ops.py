@@ -461,6 +461,37 @@ def test_sample_ties_and_extremes(V):
     assert ops.sample_tokens(torch.zeros(0, V, device=DEV), torch.zeros(0, device=DEV)).shape == (0,)
 
 
+@pytest.mark.parametrize("what", ["normal", "near 0", "far", "halves", "few values", "masked low", "one"])
+def test_sample_bf16_values(what):
+    """Rows that the counting of bf16 values meets: spread ones, many within 2^-9 of 0 (more than its list holds, too), beyond 2^9, ties at
+    every cut, masked with large negative numbers."""
+    g = gen(len(what))
+    rows, V = 6, 9001
+    x = rnd(g, rows, V, std=2.5)
+    if what == "near 0":
+        x = x * torch.tensor([1e-4, 1e-3, 4e-3, 0.02, 0.1, 0.3])[:, None]
+    elif what == "far":
+        x = x * torch.tensor([100.0, 200.0, 1e3, 1e6, 1.0, 1.0])[:, None]
+        x[4, 7], x[5, 9] = -3e38, 600.0
+    elif what == "halves":
+        x = torch.round(x * 2) / 2
+    elif what == "few values":
+        x = torch.randint(0, 3, (rows, V), generator=g).float() + torch.arange(rows)[:, None] - 3
+    elif what == "masked low":
+        x[torch.rand(rows, V, generator=g) < 0.9] = -1e9
+        x[1] = x[1].clamp(max=-520.0)
+        x[2, 1:] = -1e9
+    elif what == "one":
+        x[:] = -float("inf")
+        x[torch.arange(rows), torch.arange(rows) * 1500] = torch.tensor([3.0, 0.0, -0.001, -40.0, 1e-30, 511.0])
+    x = x.bfloat16()
+    u = torch.rand(rows, generator=g)
+    for settings in (dict(), dict(temperature=0.3), dict(top_p=0.9), dict(top_p=0.5, min_p=0.1), dict(min_p=0.02, temperature=2.0), dict(top_k=2000), dict(top_k=V - 3, top_p=0.8),
+                     dict(top_k=1500, top_p=0.999, min_p=1e-4), dict(min_p=1.0), dict(temperature=30.0, top_p=0.7)):
+        full = {**dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **settings}
+        assert ops.sample_tokens(dev(x), dev(u), **settings).cpu().tolist() == want_tokens(x, u, **full), f"{settings}"
+
+
 def test_sample_frequencies():
     """2^16 draws of one row: each token's count within six standard deviations of its probability."""
     x = torch.tensor([0.3, -1.0, 2.0, 1.9, 0.0, -3.0, 1.0])
