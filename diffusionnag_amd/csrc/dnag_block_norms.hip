@@ -36,8 +36,9 @@ template <int TPR> struct RowSum {
         if ((threadIdx.x & 63) == 0) b[threadIdx.x >> 6] = v;
         __syncthreads();
         float s = b[0];
+        const int waves = blockDim.x >> 6;             // as many as the row needs
 #pragma unroll
-        for (int w = 1; w < TPR / 64; ++w) s += b[w];
+        for (int w = 1; w < TPR / 64; ++w) s += w < waves ? b[w] : 0.f;
         return s;
     }
 };
@@ -69,8 +70,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_kernel(cons
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1;
     __shared__ float red[2][16];
     RowSum<TPR> sum{red};
-    const int lane = threadIdx.x & (TPR - 1);
-    const int64_t row = (int64_t)blockIdx.x * NT + threadIdx.x / TPR;
+    const int lane = TPR > 64 ? threadIdx.x : threadIdx.x & (TPR - 1);
+    const int64_t row = (int64_t)blockIdx.x * NT + (TPR > 64 ? 0 : threadIdx.x / TPR);
     if (row >= a.rows) return;                         // whole teams; TPR > 64: the block has one team
     int n[NV];
     f8 x[NV], y[NV];
@@ -119,13 +120,14 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_kernel(cons
 }
 
 // order of the partial sums: pre weight, post weight, pre bias, post bias (the biases for LayerNorm only)
+// (5 waves per SIMD above 4096 columns: two workgroups of up to ten waves on a CU, instead of one)
 template <class TX, class TY, int TPR, int NV, bool LN>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel(const BnArgs a) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !LN ? 5 : 1) void block_norms_grad_kernel(const BnArgs a) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1, NA = LN ? 4 : 2;
     __shared__ float red[2][16];
     __shared__ __attribute__((aligned(32))) float comb[NT > 1 ? 3 * TPR * 8 * NV : 1];
     RowSum<TPR> sum{red};
-    const int lane = threadIdx.x & (TPR - 1), team = threadIdx.x / TPR;
+    const int lane = TPR > 64 ? threadIdx.x : threadIdx.x & (TPR - 1), team = TPR > 64 ? 0 : threadIdx.x / TPR;
     int n[NV];
     f8 acc[NA][NV], dg[NV];
 #pragma unroll
@@ -344,7 +346,7 @@ namespace {
 constexpr int BN_MAX_D = 16384;
 int lanes_for(int64_t d) {                             // lanes of a team: eight columns each
     const int64_t v = ceil_div(d, 8);
-    return v <= 8 ? 8 : v <= 32 ? 32 : pow2_at_least(v, 64, 1024);
+    return v <= 8 ? 8 : v <= 16 ? 16 : v <= 32 ? 32 : pow2_at_least(v, 64, 1024);
 }
 struct BnPlan {
     int tpr, nt, nblk, S, na, cell;
@@ -357,8 +359,8 @@ BnPlan grad_plan(const dnag_block_norms_args &p) {
     q.nt = q.tpr <= 64 ? 256 / q.tpr : 1;
     q.na = p.layer_norm ? 4 : 2;
     const int64_t G = p.gate_rows, rpg = p.rows / G;
-    // two blocks of 256 lanes for every CU: fewer partial sums than a block per row, and enough rows in flight
-    const int64_t target = q.tpr <= 64 ? 512 : q.tpr <= 256 ? 1024 : q.tpr == 512 ? 512 : 256;
+    // as many blocks as the chip holds at a time, or twice that: fewer partial sums than with a block per row
+    const int64_t target = q.tpr <= 64 || q.tpr >= 512 ? 512 : 1024;
     q.S = 1;
     if (rpg >= q.nt) {
         int64_t s = ceil_div(target, G), most = ceil_div(rpg, q.nt);
@@ -401,7 +403,8 @@ BnArgs common_args(const dnag_block_norms_args &p) {
 }
 template <class TX, class TY, int TPR, int NV, bool LN>
 int launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
-    constexpr int threads = TPR <= 64 ? 256 : TPR;
+    // a team above 64 lanes is the workgroup: whole waves, as many as the row needs (4100 columns: 9, not 16)
+    const int threads = TPR <= 64 ? 256 : NV > 1 ? TPR : (int)(ceil_div(a.d, 512) * 64);
     if (grad) {
         const size_t lds = NV == 1 ? (size_t)3 * threads * 32 : 0;
         static LdsLimit limit;
@@ -414,6 +417,7 @@ template <class TX, class TY, bool LN>
 int launch_width(const BnArgs &a, int tpr, bool grad, unsigned blocks, hipStream_t st) {
     switch (tpr) {
         case 8: return launch<TX, TY, 8, 1, LN>(a, grad, blocks, st);
+        case 16: return launch<TX, TY, 16, 1, LN>(a, grad, blocks, st);
         case 32: return launch<TX, TY, 32, 1, LN>(a, grad, blocks, st);
         case 64: return launch<TX, TY, 64, 1, LN>(a, grad, blocks, st);
         case 128: return launch<TX, TY, 128, 1, LN>(a, grad, blocks, st);

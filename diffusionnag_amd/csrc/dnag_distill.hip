@@ -7,7 +7,8 @@
 // keeps its row's raw elements in registers (NV pieces of eight per lane) between the maximum, the sum and the gradient;
 // above 131072 16-bit or 65536 fp32 logits (NV = 0) the row is read again, out of the caches.  The teacher's entries are the first wave's work beside
 // that; the few elements of the gradient that hold an entry are written again, in full precision, behind the row.
-// Sums are fp32, in a fixed order; exponentials are v_exp_f32 (1 ulp) of (s - max) log2(e) / tau.
+// Sums are fp32, in a fixed order.  Exponentials are v_exp_f32 (1 ulp) of s c - R, one fused operation, with c = log2(e) / tau and R the
+// rounded c max(s): R is a reference that divides out, so its rounding does not matter.
 #include "dnag_token_common.h"
 #include <math.h>
 
@@ -22,7 +23,7 @@ struct DistillArgs {
     const float *wsum;                                 // sum of the positive weights (mean with weights) or NULL
     float scale;                                       // 1 / rows (mean without weights) or 1
     float *row_loss;                                   // [rows] or NULL: w_t tau^2 KL_t
-    float *stats;                                      // [rows][2] or NULL: maximum, sum of exponentials
+    float *stats;                                      // [rows][2] or NULL: reference R, sum of exponentials
     const float *gout;                                 // MODE 2: upstream gradient, gout[t * gstep]
     int64_t gstep;
     void *grad;
@@ -40,10 +41,12 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
     typedef typename Vec8<T>::type raw8;
     extern __shared__ char lds[];
     __shared__ float red[33];                          // pairs of the waves; [32]: the teacher's maximum
-    float *tp = (float *)lds + (size_t)(threadIdx.x / TPR) * 2 * a.K;      // the team's entries: probability, index
+    float *tp = (float *)lds + (size_t)(TPR > 64 ? 0 : threadIdx.x / TPR) * 3 * a.K;      // the team's entries: teacher's logit, index, student's logit
     int *ti = (int *)(tp + a.K);
-    const int lane = threadIdx.x & (TPR - 1);
-    const int64_t row = (int64_t)blockIdx.x * NT + threadIdx.x / TPR;
+    float *ts = tp + 2 * a.K;
+    // a team above 64 lanes is the workgroup, which has as many waves as the row needs
+    const int tpr = TPR > 64 ? (int)blockDim.x : TPR, lane = TPR > 64 ? threadIdx.x : threadIdx.x & (TPR - 1);
+    const int64_t row = (int64_t)blockIdx.x * NT + (TPR > 64 ? 0 : threadIdx.x / TPR);
     if (row >= a.rows) return;
     const T *s = (const T *)a.logits + row * a.ld;
     T *g = MODE > 0 ? (T *)a.grad + row * a.V : nullptr;
@@ -51,7 +54,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
     const bool on = w > 0.f;
     auto zero_row = [&]() {
         if constexpr (MODE > 0)
-            for (int c = lane * 8; c < a.V; c += TPR * 8) store8_n(g + c, splat8(0.f), a.V - c);
+            for (int c = lane * 8; c < a.V; c += tpr * 8) store8_n(g + c, splat8(0.f), a.V - c);
         if (MODE < 2 && lane == 0) {
             if (a.row_loss) a.row_loss[row] = 0.f;
             if (a.stats) { a.stats[2 * row] = 0.f; a.stats[2 * row + 1] = 1.f; }
@@ -63,7 +66,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
     if constexpr (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * TPR + lane) * 8, n = a.V - c;
+            const int c = (j * tpr + lane) * 8, n = a.V - c;
             if (n >= 8) x[j] = load8_raw(s + c);
             else
 #pragma unroll
@@ -81,6 +84,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
                                                                                                           : (float)((const tf16 *)a.tlogits)[at];
             tp[k] = in ? z : -INFINITY;
             ti[k] = in ? (int)i : -1;
+            ts[k] = in ? (float)s[i] : 0.f;
             if (in) tmax = z != z || tmax != tmax ? NAN : fmaxf(tmax, z);          // a NaN among the entries stays one
         }
 #pragma unroll
@@ -94,68 +98,65 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
     }
     if constexpr (TPR > 64) { __syncthreads(); tmax = red[32]; }
     if (tmax == -INFINITY) { zero_row(); return; }     // no entry (the same for the whole team)
-    // Every lane takes its exponentials relative to its own largest logit `tm`, in fp32 (MODE 1 keeps them for the gradient), so that one
-    // exchange of (maximum, sum) pairs gives the row's: exp(s - m) = exp(s - tm) exp(tm - m).
-    float m, sum, tm = LOW, own = 0.f;
+    // Every lane takes its exponentials relative to its own reference `tr`, in fp32 (MODE 1 keeps them for the gradient), so that one
+    // exchange of (reference, sum) pairs gives the row's.
     constexpr bool KEEP = MODE == 1 && NV > 0 && NV <= 8;      // 16 pieces: their registers would spill
+    float ref, sum, tr = LOW, own = 0.f;
     f8 ex[KEEP ? NV : 1];
-    if constexpr (MODE == 2) { m = a.stats[2 * row]; sum = a.stats[2 * row + 1]; }
-    else {
-        auto exps = [&](f8 v) {
-            v = (v - tm) * a.c2;
+    auto exps = [&](f8 v, float r) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = exp2_hw(v[e]);
-            return v;
-        };
+        for (int e = 0; e < 8; ++e) v[e] = exp2_hw(fmaf(v[e], a.c2, -r));
+        return v;
+    };
+    if constexpr (MODE == 2) { ref = a.stats[2 * row]; sum = a.stats[2 * row + 1]; }
+    else {
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) tm = fmaxf(tm, max8(widen<T>(x[j])));
+            for (int j = 0; j < NV; ++j) tr = fmaxf(tr, max8(widen<T>(x[j])));
+            tr = fmaxf(tr * a.c2, LOW);                // (a lane without logits: LOW)
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const f8 v = exps(widen<T>(x[j]));
+                const f8 v = exps(widen<T>(x[j]), tr);
                 own += sum8(v);
                 if constexpr (KEEP) ex[j] = v;
             }
         } else
-            for (int c = lane * 8; c < a.V; c += TPR * 8) {
+            for (int c = lane * 8; c < a.V; c += tpr * 8) {
                 const f8 v = load8_n(s + c, a.V - c, -INFINITY);
-                const float nm = fmaxf(tm, max8(v));
-                own *= exp2_hw((tm - nm) * a.c2);
-                tm = nm;
-                own += sum8(exps(v));
+                const float nr = fmaxf(tr, max8(v) * a.c2);
+                own *= exp2_hw(tr - nr);
+                tr = nr;
+                own += sum8(exps(v, tr));
             }
-        m = tm;
+        ref = tr;
 #pragma unroll
-        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        sum = own * exp2_hw((tm - m) * a.c2);
+        for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
+        sum = own * exp2_hw(tr - ref);
 #pragma unroll
         for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if constexpr (TPR > 64) {
-            if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = m; red[2 * (threadIdx.x >> 6) + 1] = sum; }
+            if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = ref; red[2 * (threadIdx.x >> 6) + 1] = sum; }
             __syncthreads();
-            float all = red[0];
-#pragma unroll
-            for (int w = 1; w < TPR / 64; ++w) all = fmaxf(all, red[2 * w]);
-            m = all;
+            const int waves = tpr >> 6;
+            for (int w = 0; w < waves; ++w) ref = fmaxf(ref, red[2 * w]);
             sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < TPR / 64; ++w) sum += red[2 * w + 1] * exp2_hw((red[2 * w] - m) * a.c2);
+            for (int w = 0; w < waves; ++w) sum += red[2 * w + 1] * exp2_hw(red[2 * w] - ref);
         }
     }
     if constexpr (MODE < 2) {
         if (lane < TW) {
-            const float ltsum = logf(tsum), lsum = logf(sum), it = 1.0f / a.tau;
+            const float ltsum = log2f(tsum), lsum = log2f(sum);
             float l = 0.f;
             for (int k = lane; k < a.K; k += TW) {
                 if (ti[k] < 0) continue;
-                const float u = (tp[k] - tmax) * it, p = exp2_hw((tp[k] - tmax) * a.c2) / tsum;
-                if (!(p == 0.f)) l += p * ((u - ltsum) - (((float)s[ti[k]] - m) * it - lsum));
+                const float u = (tp[k] - tmax) * a.c2, p = exp2_hw(u) / tsum;
+                if (!(p == 0.f)) l += p * ((u - ltsum) - (fmaf(ts[k], a.c2, -ref) - lsum));
             }
 #pragma unroll
             for (int o = TW / 2; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
             if (lane == 0) {
-                if (a.row_loss) a.row_loss[row] = a.tau * a.tau * w * l;
-                if (a.stats) { a.stats[2 * row] = m; a.stats[2 * row + 1] = sum; }
+                if (a.row_loss) a.row_loss[row] = a.tau * a.tau * w * (l * 0.69314718056f);
+                if (a.stats) { a.stats[2 * row] = ref; a.stats[2 * row + 1] = sum; }
             }
         }
     }
@@ -164,27 +165,21 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
         if (a.wsum) f /= *a.wsum;                      // positive: this row's weight is part of it
         if constexpr (MODE == 2) f *= a.gout[row * a.gstep];
         const float fq = f / sum;
-        auto put = [&](int c, f8 v) {
-            v = (v - m) * a.c2;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = exp2_hw(v[e]);
-            store8_n(g + c, v * fq, a.V - c);
-        };
         if constexpr (KEEP) {
-            const float ft = fq * exp2_hw((tm - m) * a.c2);
+            const float ft = fq * exp2_hw(tr - ref);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = (j * TPR + lane) * 8;
+                const int c = (j * tpr + lane) * 8;
                 if (c < a.V) store8_n(g + c, ex[j] * ft, a.V - c);
             }
         } else if constexpr (NV > 0) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = (j * TPR + lane) * 8;
-                if (c < a.V) put(c, widen<T>(x[j]));
+                const int c = (j * tpr + lane) * 8;
+                if (c < a.V) store8_n(g + c, exps(widen<T>(x[j]), ref) * fq, a.V - c);
             }
         } else
-            for (int c = lane * 8; c < a.V; c += TPR * 8) put(c, load8_n(s + c, a.V - c));
+            for (int c = lane * 8; c < a.V; c += tpr * 8) store8_n(g + c, exps(load8_n(s + c, a.V - c), ref) * fq, a.V - c);
         if constexpr (TPR > 64) __syncthreads();       // the row is written before its entries are
         else wave_fence();
         if (lane < TW)
@@ -195,7 +190,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
                 bool first = true;
                 for (int j = 0; j < a.K; ++j)
                     if (ti[j] == i) { z += exp2_hw((tp[j] - tmax) * a.c2); first &= j >= k; }
-                if (first) g[i] = (T)(f * (exp2_hw(((float)s[i] - m) * a.c2) / sum - z / tsum));
+                if (first) g[i] = (T)(f * (exp2_hw(fmaf(ts[k], a.c2, -ref)) / sum - z / tsum));
             }
     }
 }
@@ -278,7 +273,9 @@ DistillArgs fill(const dnag_distill_args &p) {
 template <class T, int MODE, int TPR, int NV>
 int launch(const DistillArgs &a, hipStream_t st) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1;
-    hipLaunchKernelGGL((distill_kernel<T, TPR, NV, MODE>), dim3((unsigned)ceil_div(a.rows, NT)), dim3(TPR <= 64 ? 256 : TPR), (size_t)NT * a.K * 8, st, a);
+    const int64_t lanes = NV > 0 ? ceil_div(a.V, 8 * NV) : TPR;        // a team above 64 lanes: whole waves, as many as the row fills
+    const unsigned threads = TPR <= 64 ? 256 : (unsigned)(ceil_div(lanes, 64) * 64);
+    hipLaunchKernelGGL((distill_kernel<T, TPR, NV, MODE>), dim3((unsigned)ceil_div(a.rows, NT)), dim3(threads), (size_t)NT * a.K * 12, st, a);
     TOK_TRY(hipGetLastError());
     return 0;
 }
@@ -291,8 +288,6 @@ int launch_size(const DistillArgs &a, hipStream_t st) {
     if (V <= 2048) return launch<T, MODE, 64, 4>(a, st);
     if (V <= 8192) return launch<T, MODE, 256, 4>(a, st);
     if (V <= 32768) return launch<T, MODE, 512, 8>(a, st);
-    // the loss alone: two workgroups of 512 on a CU, one of which waits for its row while the other sums (1000 x 50001 fp16: 37 us with one of 1024)
-    if (V <= 65536 && MODE == 0 && sizeof(T) == 2) return launch<T, MODE, 512, sizeof(T) == 2 ? 16 : 8>(a, st);
     if (V <= 65536) return launch<T, MODE, 1024, 8>(a, st);
     if (sizeof(T) == 2 && V <= 131072) return launch<T, MODE, 1024, sizeof(T) == 2 ? 16 : 0>(a, st);
     return launch<T, MODE, 1024, 0>(a, st);
