@@ -120,9 +120,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_kernel(cons
 }
 
 // order of the partial sums: pre weight, post weight, pre bias, post bias (the biases for LayerNorm only)
-// (5 waves per SIMD above 4096 columns: two workgroups of up to ten waves on a CU, instead of one)
 template <class TX, class TY, int TPR, int NV, bool LN>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !LN ? 5 : 1) void block_norms_grad_kernel(const BnArgs a) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void block_norms_grad_kernel(const BnArgs a) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1, NA = LN ? 4 : 2;
     __shared__ float red[2][16];
     __shared__ __attribute__((aligned(32))) float comb[NT > 1 ? 3 * TPR * 8 * NV : 1];
@@ -159,10 +158,13 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !L
     auto post_weight = [&](int j) { if constexpr (HELD) return held_at(0); else return small(a.pw, 2, (j * TPR + lane) * 8, j, 1.f); };
     auto pre_weight = [&](int j) { if constexpr (HELD) return held_at(1); else return small(a.qw, 4, (j * TPR + lane) * 8, j, 1.f); };
     auto gate_of = [&](int j, size_t g0) { if constexpr (HELD) return held_at(2); else return small(a.gate, 1, g0 + (j * TPR + lane) * 8, j, 1.f); };
-    auto one_row = [&](int64_t row, size_t g0) __attribute__((always_inline)) {      // as a call its sums would live in memory
-        f8 x[NV], y[NV], gx[NV], gh[NV];
-        typename Vec8<TX>::type rx[NV], rgx[NV];
-        typename Vec8<TY>::type ry_[NV], rgh[NV];
+    // Above 4096 columns a CU holds one workgroup: the next row is asked for as soon as this one's registers are free (8192 rows of bf16,
+    // 5120 columns: 207 us without, 181 with; 8192 columns: 265 and 212).  Below, the registers that takes would cost a second
+    // workgroup, which hides more; with fp32 rows and in the layer's form they would go to scratch.
+    constexpr bool AHEAD = TPR == 1024 && NV == 1 && !LN && sizeof(TX) == 2;
+    typename Vec8<TX>::type rx[NV], rgx[NV];
+    typename Vec8<TY>::type ry_[NV], rgh[NV];
+    auto fetch = [&](int64_t row) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * TPR + lane) * 8;
@@ -173,6 +175,10 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !L
                 if (a.gh) rgh[j] = load8_raw_n((const TY *)a.gh + row * a.ghs + c, n[j]);
             }
         }
+    };
+    auto one_row = [&](int64_t row, size_t g0, int64_t next) __attribute__((always_inline)) {      // as a call its sums would live in memory
+        f8 x[NV], y[NV], gx[NV], gh[NV];
+        if constexpr (!AHEAD) fetch(row);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             x[j] = n[j] > 0 ? widen<TX>(rx[j]) : splat8(0.f);
@@ -180,6 +186,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !L
             gx[j] = n[j] > 0 && a.gx ? widen<TX>(rgx[j]) : splat8(0.f);
             gh[j] = n[j] > 0 && a.gh ? widen<TY>(rgh[j]) : splat8(0.f);
         }
+        if constexpr (AHEAD) if (next >= 0) fetch(next);
         float ry = 0.f;
         if (a.y) {
             ry = normalise<LN>(y, n, sum, a.eps, a.inv_d);
@@ -282,8 +289,11 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR == 1024 && NV == 1 && !L
         const int64_t end = (g + 1) * a.rpg, r0 = g * a.rpg + s * a.split_rows, r1 = few || r0 + a.split_rows > end ? end : r0 + a.split_rows;
         clear();
         if constexpr (HELD) if (g < a.G) hold(2, small(a.gate, 1, (size_t)g * a.d + lane * 8, 0, 1.f));
-        if (g < a.G)
-            for (int64_t r = r0 + sub; r < r1; r += few ? a.cell : NT) one_row(r, (size_t)g * a.d);
+        if (g < a.G) {
+            const int64_t step = few ? a.cell : NT;
+            if constexpr (AHEAD) if (r0 + sub < r1) fetch(r0 + sub);
+            for (int64_t r = r0 + sub; r < r1; r += step) one_row(r, (size_t)g * a.d, r + step < r1 ? r + step : -1);
+        }
         if (!a.dgate) continue;
         if (few) {
             for (int o = TPR; o < a.cell * TPR; o <<= 1)
@@ -360,7 +370,7 @@ BnPlan grad_plan(const dnag_block_norms_args &p) {
     q.na = p.layer_norm ? 4 : 2;
     const int64_t G = p.gate_rows, rpg = p.rows / G;
     // as many blocks as the chip holds at a time, or twice that: fewer partial sums than with a block per row
-    const int64_t target = q.tpr <= 64 || q.tpr >= 512 ? 512 : 1024;
+    const int64_t target = q.tpr <= 64 || q.tpr == 512 ? 512 : q.tpr > 512 ? 256 : 1024;
     q.S = 1;
     if (rpg >= q.nt) {
         int64_t s = ceil_div(target, G), most = ceil_div(rpg, q.nt);
