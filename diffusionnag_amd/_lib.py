@@ -38,7 +38,7 @@ EXPORTS = (
     "dnag_embed_forward", "dnag_embed_grad_workspace_bytes", "dnag_embed_grad",
     "dnag_block_norms_args_bytes", "dnag_block_norms_grad_workspace_bytes", "dnag_block_norms_forward", "dnag_block_norms_grad",
     "dnag_distill_args_bytes", "dnag_distill_workspace_bytes", "dnag_distill_loss", "dnag_distill_loss_grad", "dnag_distill_backward",
-    "dnag_sample_args_bytes", "dnag_sample_tokens",
+    "dnag_sample_args_bytes", "dnag_sample_workspace_bytes", "dnag_sample_tokens",
 )
 
 
@@ -135,13 +135,14 @@ class DistillArgsC(C.Structure):
 # the same structs for packing a call's arguments in one go (a third of the time of setting their fields)
 BLOCK_NORMS_LAYOUT = struct.Struct("@3q5i2f7P2q4P2q8PNP")
 DISTILL_LAYOUT = struct.Struct("@3q5if9PNP")
-SAMPLE_LAYOUT = struct.Struct("@3q2i3d8P")
+SAMPLE_LAYOUT = struct.Struct("@3q2i3d8PNP")
 
 
 class SampleArgsC(C.Structure):
     _fields_ = ([(n, C.c_int64) for n in ("rows", "vocab", "logits_stride")] + [("dtype", C.c_int32), ("top_k", C.c_int32)] +
                 [(n, C.c_double) for n in ("temperature", "top_p", "min_p")] +
-                [(n, C.c_void_p) for n in ("logits", "u", "temperature_rows", "top_k_rows", "top_p_rows", "min_p_rows", "out", "stream")])
+                [(n, C.c_void_p) for n in ("logits", "u", "temperature_rows", "top_k_rows", "top_p_rows", "min_p_rows", "out", "workspace")] +
+                [("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)])
 
 _lib: Optional[C.CDLL] = None
 
@@ -242,7 +243,7 @@ def load() -> C.CDLL:
              ("dnag_block_norms_forward", "dnag_block_norms_grad")),
             (DistillArgsC, DISTILL_LAYOUT, "dnag_distill_args_bytes", "dnag_distill_workspace_bytes",
              ("dnag_distill_loss", "dnag_distill_loss_grad", "dnag_distill_backward")),
-            (SampleArgsC, SAMPLE_LAYOUT, "dnag_sample_args_bytes", None, ("dnag_sample_tokens",))):
+            (SampleArgsC, SAMPLE_LAYOUT, "dnag_sample_args_bytes", "dnag_sample_workspace_bytes", ("dnag_sample_tokens",))):
         getattr(lib, size).restype = sz
         if not getattr(lib, size)() == C.sizeof(args) == layout.size:
             raise ImportError(f"{LIB_PATH}: {size}() is {getattr(lib, size)()}, this binding has {C.sizeof(args)} and {layout.size}; rebuild the library")

@@ -227,9 +227,10 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict_
     }
 }
 
-// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` (at most TPR, or 64) entries.  The lanes fetch the
+// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` (8 to 64, at most TPR) entries.  The lanes fetch the
 // entries at once, one each, so that the rows' addresses are known before the first row is asked for; eight rows are
-// under way at a time (fetching four entries, then their rows, in turn: 94 us for 32768 x 2048 bf16; this: 41).
+// under way at a time (fetching four entries, then their rows, in turn: 94 us for 32768 x 2048 bf16; this: 55, 2.4 TB/s of the
+// gradient's rows).
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t rows,
                                                         const T *__restrict__ grad, int64_t gstride, uint32_t V, int d, float scale, int chunk, int ntile,

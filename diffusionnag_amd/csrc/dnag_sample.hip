@@ -12,14 +12,17 @@
 // 2^-45.9 off at most, below the weights' step.  2^-40 is below what a uniform fp32 number resolves.
 //
 // One workgroup per row, which reads the row again (out of the caches) for each of its passes; bound by the instructions per
-// logit, not by HBM, so the passes are few and the exact work falls on few logits:
-//   top-k of at most as many as there are lanes: the k-th largest of the lanes' own maxima is no larger than the k-th largest
-//     logit, so the logits from there on (little more than k) hold all candidates: they are sorted in LDS and everything else --
-//     top-p, min-p, the draw -- happens on that list.
+// logit, not by HBM, so the passes are few and the exact work falls on few logits (256 rows of 128000 bf16: k = 50 30 us, top-p
+// 59 us, no cut 50 us; the row's bytes alone 13 us):
+//   top-k of few: the k-th largest of the lanes' own maxima is no larger than the k-th largest logit, so the logits from there on
+//     (little more than k) hold all candidates: they are sorted in LDS and everything else -- top-p, min-p, the draw -- happens on
+//     that list.
+//   bf16 with another cut: the values are counted, and exponentials, sums and cuts are taken over the values that there are.
 //   otherwise a cut (top-k, top-p) is found by a histogram over 2048 equal steps of (max - l) / T; the logits in the step where
 //     the sum passes its goal are sorted (or, where they are more than the list holds, divided by eleven, eleven and ten bits of
 //     their ordered bit pattern and then by index).  The draw sums pieces of 512 logits, then looks into one piece.
-// Rows of at most 64 logits take a team of lanes each and rank by comparing all pairs.
+// Rows of at most 64 logits take a team of lanes each and rank by comparing all pairs.  For few long rows the maxima of groups of logits
+// and the weights are taken by many workgroups first (split_rows, below).
 #include "dnag_token_common.h"
 #include <float.h>
 #include <math.h>
@@ -29,6 +32,7 @@
 #define SMP_BITS 40
 #define SMP_MAX_V (1 << 20)      // sums stay below 2^60
 #define SMP_LIST 2048            // logits that are sorted in LDS
+#define SMP_GROUP 128            // logits whose maximum is kept
 
 typedef unsigned long long u64;
 
@@ -42,6 +46,8 @@ struct SampleArgs {
     double temperature1, top_p1, min_p1;               // where NULL
     int top_k1;
     int64_t *out;
+    char *ws;                                          // few long rows: per row hist[SMP_BINS], a sum per piece, a maximum per group
+    int64_t ws_row;
 };
 struct RowSet { double c, p, minw; int k; bool greedy; };      // c = log2(e) / T; minw = min_p 2^40
 __device__ __forceinline__ RowSet row_set(const SampleArgs &a, int64_t row) {
@@ -57,6 +63,14 @@ __device__ __forceinline__ RowSet row_set(const SampleArgs &a, int64_t row) {
 }
 // a logit as compared: NaN counts as -inf, -0 as +0
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+__device__ __forceinline__ bool cuts_by_rank(const RowSet &s, int V) { return s.k > 0 && s.k < V; }
+// The largest k that is sorted in a short list; beyond it the list's sorting costs more than cutting at a histogram.  Both in us, 64 rows
+// of 100 logits, k = 20: 20 and 10; of 2000, 20: 10 and 10, 100: 17 and 10; of 8192, 100: 15 and 17, 200: 23 and 17; of 128000,
+// 256: 35 and 50 (bf16), 400: 52 and 63 (fp32).
+__host__ __device__ inline int short_list_k(int64_t V, bool counted) {
+    const int most = counted ? 256 : 512, k = (int)(V / 256 < most ? V / 256 : most);
+    return V <= 4096 ? (int)(V / 64) : k > 128 ? k : 128;
+}
 // order of the bit patterns = order of the values
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -84,6 +98,39 @@ __device__ __forceinline__ double raw_weight(float x, double m, double c) {
 __device__ __forceinline__ u64 whole_weight(double v) {        // v in [0, 2^41): rounded by the addition's own rounding
     return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull;
 }
+__device__ __forceinline__ float value_of_key(uint32_t k) { return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu)); }
+// a row's weights and its steps of (max - l) / T; an infinite maximum leaves its equals alone: they weigh 1, everything else is
+// below any cut
+struct Weigh {
+    float m;
+    double md, c;
+    bool inf;
+    float per_step;
+    __device__ __forceinline__ void set(float top, double scale) {
+        m = top; c = scale; inf = m == INFINITY; md = inf ? 0.0 : (double)m;
+        per_step = fminf((float)(c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE)), 1e30f);
+    }
+    __device__ __forceinline__ double raw(float x) const { return raw_weight(inf ? (x == m ? 0.f : -INFINITY) : x, md, c); }
+    __device__ __forceinline__ u64 whole(float x) const { return whole_weight(raw(x)); }
+    // never falls as x falls; the step is its whole part
+    __device__ __forceinline__ float step(float x) const { return inf ? (x == m ? 0.f : SMP_BINS - 1.f) : fminf((m - x) * per_step, SMP_BINS - 1.f); }
+    // min-p is a cut too: the smallest logit that weighs enough, by halving the ordered bit patterns up to the maximum's
+    __device__ __forceinline__ float min_p_cut(double minw) const {
+        uint32_t lo = 0x007fffffu, hi = ordered(m);    // lo: -inf, too light; hi: weighs enough, or is the largest anyway
+        auto enough = [&](uint32_t key) { return raw(value_of_key(key)) >= minw; };
+        const uint32_t near = ordered(clean((float)(md + (log2(minw) - SMP_BITS) / c)));       // almost always within two patterns
+        if (near > lo + 2 && near + 2 < hi) {
+            if (enough(near + 2)) hi = near + 2;
+            if (!enough(near - 2)) lo = near - 2;
+        }
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (enough(mid)) hi = mid;
+            else lo = mid;
+        }
+        return value_of_key(hi);
+    }
+};
 __device__ __forceinline__ u64 goal_of(double p, u64 total) {          // smallest whole number >= p total, 1 at least
     const double r = ceil(p * (double)total);
     return r >= 1.0 ? (r < (double)total ? (u64)r : total) : 1;
@@ -141,10 +188,100 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const SampleArgs a, i
     if (lane == 0) a.out[row] = token;
 }
 
+// ---- few long rows: what the row's workgroup would read them for, by many ------------------------------------------------
+__host__ __device__ inline int64_t ws_pieces(int64_t V) { return (V + 511) / 512; }
+__host__ __device__ inline int64_t ws_groups(int64_t V) { return (V + SMP_GROUP - 1) / SMP_GROUP; }
+struct RowSpace {
+    u64 *hist, *piece;
+    float *top;                                        // the largest logit of every SMP_GROUP
+    __device__ __forceinline__ RowSpace(const SampleArgs &a, int64_t row) {
+        hist = (u64 *)(a.ws + row * a.ws_row);
+        piece = hist + SMP_BINS;
+        top = (float *)(piece + ws_pieces(a.V));
+    }
+};
+// eight logits from c on as they are; past the end the row's last eight, with what lies before c set to -inf
+template <class T> __device__ __forceinline__ f8 last8(typename Vec8<T>::type raw, int c, int V) {
+    f8 v = widen<T>(raw);
+    if (c + 8 > V) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (e < 8 - (V - c)) v[e] = -INFINITY;
+    }
+    return v;
+}
+template <class T>
+__global__ __launch_bounds__(256) void sample_groups_kernel(const SampleArgs a) {
+    const RowSpace w(a, blockIdx.y);
+    const T *l = (const T *)a.logits + blockIdx.y * a.ld;
+    const int i = blockIdx.x * 256 + threadIdx.x, c = i * 8;
+    for (int b = i; b < SMP_BINS; b += gridDim.x * 256) w.hist[b] = 0;
+    const f8 v = last8<T>(load8_raw(l + (c + 8 <= a.V ? c : a.V - 8)), c, a.V);
+    float m = fmaxf(-INFINITY, max8(v));
+    m = team_max<SMP_GROUP / 8>(m);
+    if (c < a.V && (threadIdx.x & (SMP_GROUP / 8 - 1)) == 0) w.top[c / SMP_GROUP] = clean(m);
+}
+// Without a cut by rank: with top-p the histogram, otherwise every piece's kept weight.  The sums are whole numbers, so neither depends on order.
+template <class T>
+__global__ __launch_bounds__(256) void sample_weights_kernel(const SampleArgs a) {
+    constexpr int EACH = 2;                            // pieces of a wave
+    typedef typename Vec8<T>::type raw8;
+    __shared__ u64 hist[SMP_BINS];
+    __shared__ float wf[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V;
+    const RowSet s = row_set(a, blockIdx.y);
+    if (s.greedy || cuts_by_rank(s, V)) return;
+    const RowSpace w(a, blockIdx.y);
+    const T *l = (const T *)a.logits + blockIdx.y * a.ld;
+    const int p0 = (blockIdx.x * 4 + wave) * EACH;
+    raw8 raw[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int c = (p0 + j) * 512 + lane * 8;
+        raw[j] = load8_raw(l + (c + 8 <= V ? c : V - 8));
+    }
+    const bool nucleus = !__is_same(T, tbf16) && s.p < 1.0;    // bf16 rows are not split where top-p is asked for
+    if (nucleus) for (int b = tid; b < SMP_BINS; b += 256) hist[b] = 0;
+    float m = -INFINITY;
+    const int groups = (int)ws_groups(V);
+    for (int g = tid; g < groups; g += 256) m = fmaxf(m, w.top[g]);
+    m = team_max<64>(m);
+    if (lane == 0) wf[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(wf[0], wf[1]), fmaxf(wf[2], wf[3]));
+    if (m == -INFINITY) return;
+    Weigh weigh;
+    weigh.set(m, s.c);
+    if (nucleus) {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const f8 v = last8<T>(raw[j], (p0 + j) * 512 + lane * 8, V);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float q = weigh.step(v[e]);
+                if (q < SMP_BINS - 1.f) atomicAdd(&hist[(int)q], weigh.whole(v[e]));
+            }
+        }
+        __syncthreads();
+        for (int b = tid; b < SMP_BINS; b += 256) if (hist[b]) atomicAdd(&w.hist[b], hist[b]);
+        return;
+    }
+    const float from = s.minw > 0.0 ? weigh.min_p_cut(s.minw) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const f8 v = last8<T>(raw[j], (p0 + j) * 512 + lane * 8, V);
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += weigh.whole(v[e] >= from ? v[e] : -INFINITY);
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (lane == 0 && (p0 + j) * 512 < V) w.piece[p0 + j] = sum;
+    }
+}
+
 // ---- one workgroup per row -----------------------------------------------------------------------------------------------
 struct Cut { float x; int at; };   // kept: larger logits, and equal ones up to index `at`
 
-template <class T, int NTHR>
+// SPLIT: sample_groups_kernel and, where it applies, sample_weights_kernel have run
+template <class T, int NTHR, bool SPLIT>
 __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     constexpr int NW = NTHR / 64, PER = SMP_BINS / NTHR;
     constexpr bool COUNTED = __is_same(T, tbf16);
@@ -165,7 +302,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // f(first index, eight logits as they are), called by whole waves: a lane past the end has -inf, and the row's last piece
     // that is shorter than eight comes as the row's last eight with what was seen before set to -inf.  A rolled loop with three
     // pieces under way ahead of the one that is worked on: a workgroup runs through each pass once, so what counts is the code's size (with
-    // the pieces unrolled the passes waited for instructions: 256 rows of 128000 with top-p 114 us, rolled 67).
+    // the pieces unrolled the passes waited for instructions).
     auto each8 = [&](auto f) {
         typedef typename Vec8<T>::type raw8;
         constexpr int STEP = NTHR * 8;
@@ -178,20 +315,15 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             r0 = r1;
             r1 = r2;
             r2 = ask(c + 3 * STEP);
-            f8 v = widen<T>(now);
-            if (c + 8 > V) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) if (e < 8 - (V - c)) v[e] = -INFINITY;
-            }
-            f(c + 8 <= V ? c : V - 8, v);
+            f(c + 8 <= V ? c : V - 8, last8<T>(now, c, V));
         }
     };
+    const RowSpace ws_row(a, row);
+    const int groups = (int)ws_groups(V);
     float m = -INFINITY;                               // the row's largest logit
-    double md = 0.0;
-    bool inf = false;
-    // an infinite maximum leaves its equals alone: they weigh 1, everything else is below any cut
-    auto weight_raw = [&](float x) { return raw_weight(inf ? (x == m ? 0.f : -INFINITY) : x, md, s.c); };
-    auto weight = [&](float x) -> u64 { return whole_weight(weight_raw(x)); };
+    Weigh weigh;
+    auto weight_raw = [&](float x) { return weigh.raw(x); };
+    auto weight = [&](float x) { return weigh.whole(x); };
     auto wave_scan = [&](u64 v) {                      // inclusive
         for (int o = 1; o < 64; o <<= 1) { const u64 b = __shfl_up(v, o, 64); if (lane >= o) v += b; }
         return v;
@@ -208,18 +340,26 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     };
     // The list: (ordered bits, ~index) in hist[0 .. n), sorted to falling logits and rising indices.
     auto entry = [&](float x, int i) { return (u64)ordered(x) << 32 | (uint32_t)~i; };
-    auto value_of = [&](u64 e) { const uint32_t k = (uint32_t)(e >> 32); return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu)); };
+    auto value_of = [&](u64 e) { return value_of_key((uint32_t)(e >> 32)); };
     auto index_of = [&](u64 e) { return (int)~(uint32_t)e; };
     auto sort_falling = [&](int n) {
         __syncthreads();
-        if (n <= (NTHR < 512 ? NTHR : 512)) {          // by counting what is larger (no barriers between steps)
-            const u64 x = tid < n ? hist[tid] : 0;
+        if (n <= (NTHR < 512 ? NTHR : 512)) {          // by counting what is larger (no barriers between steps), `parts` lanes for each
+            int shift = 0;
+            while (shift < 6 && (n << (shift + 1)) <= NTHR) ++shift;
+            if (shift < 2) shift = 0;
+            const int i = tid >> shift, parts = 1 << shift;
+            const u64 x = i < n ? hist[i] : 0;
             int r = 0;
-            if (tid < n)
+            if (shift == 0) {
+                if (i < n)
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) { const u64 y = hist[j]; r += y > x || (y == x && j < tid); }
+                    for (int j = 0; j < n; ++j) { const u64 y = hist[j]; r += y > x || (y == x && j < i); }
+            } else if (i < n)
+                for (int j = tid & (parts - 1); j < n; j += parts) { const u64 y = hist[j]; r += y > x || (y == x && j < i); }
+            for (int o = 1; o < parts; o <<= 1) r += __shfl_xor(r, o, 64);
             __syncthreads();
-            if (tid < n) hist[r] = x;
+            if (i < n && !(tid & (parts - 1))) hist[r] = x;
             __syncthreads();
             return;
         }
@@ -240,27 +380,42 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     auto collect = [&](float from, float to, auto take) {  // logits in [from, to] that `take` wants, in any order; their number (the list may hold fewer)
         from = fmaxf(from, -FLT_MAX);                  // never -inf: neither drawn nor there (each8)
         __syncthreads();
-        if (tid == 0) listed = 0;
+        if (tid == 0) { listed = 0; at_found = 0; }
         __syncthreads();
-        each8([&](int c, const f8 &v) {
+        auto look = [&](int c, const f8 &v) {
             if (!(max8(v) >= from)) return;
             uint32_t hit = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) hit |= (v[e] >= from && v[e] <= to ? 1u : 0u) << e;
             for (; hit; hit &= hit - 1) {              // few
-                const int i = c + __ffs(hit) - 1;
-                const float x = clean((float)l[i]);
+                const int b = __ffs(hit) - 1, i = c + b;
+                float x = v[0];                        // chosen among the registers: the wave would wait for a load
+#pragma unroll
+                for (int e = 1; e < 8; ++e) x = e == b ? v[e] : x;
+                x = clean(x);
                 if (!take(x, i)) continue;
                 const int at = atomicAdd(&listed, 1);
                 if (at < SMP_LIST) hist[at] = entry(x, i);
             }
-        });
+        };
+        if constexpr (SPLIT) {                         // only the groups that reach so far
+            int *group = (int *)&queue[0][0];
+            static_assert(SMP_MAX_V / SMP_GROUP <= NW * 512, "the groups share the queue's memory");
+            for (int g = tid; g < groups; g += NTHR)
+                if (ws_row.top[g] >= from) group[atomicAdd(&at_found, 1)] = g;
+            __syncthreads();
+            const int n = at_found;
+            constexpr int TEAM = SMP_GROUP / 8;
+            for (int q = tid / TEAM; q < n; q += NTHR / TEAM) {
+                const int c = group[q] * SMP_GROUP + (tid & (TEAM - 1)) * 8;
+                if (c < V) look(c + 8 <= V ? c : V - 8, last8<T>(load8_raw(l + (c + 8 <= V ? c : V - 8)), c, V));
+            }
+        } else each8(look);
         __syncthreads();
         return listed;
     };
     Cut cut{-INFINITY, -1};                            // everything that can be drawn
-    // top-k on a short list, below (a longer list's sorting costs more than counting bf16 values: k = 1000 of 128000, 86 and 52 us)
-    const bool short_list = s.k > 0 && s.k < V && s.k <= (COUNTED && NTHR == 1024 ? 256 : NTHR);
+    const bool short_list = s.k > 0 && s.k < V && s.k <= short_list_k(V, COUNTED);
     bool done = false;                                 // `cut` is final and `piece` holds the kept weights' sums
     const int pieces = (V + 511) / 512;
     auto inside = [&](const Cut &c, float x, int i) { return x > c.x || (x == c.x && i <= c.at); };
@@ -268,8 +423,9 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // A row of bf16 logits holds few different values.  Those of magnitude 2^-9 .. 2^9 are counted (4608 slots in falling order), the
     // exponentials, sums and cuts are taken over the slots, and the draw looks its weights up.  What is nearer to 0 (slot HALF)
     // is listed and weighed one by one.  Rows that do not fit -- a logit from 512 on, a list that is too short, a cut between the
-    // listed ones -- go the general way.  256 rows of 128000, top-p: 110 us the general way, 46 this way.
-    if constexpr (sizeof(T) == 2 && NTHR == 1024 && COUNTED) {
+    // listed ones -- go the general way.  256 rows of 128000, top-p with min-p: 120 us the general way, 69 this way.
+    const bool ranks = cuts_by_rank(s, V);
+    if constexpr (NTHR == 1024 && COUNTED && !SPLIT) {
         constexpr int HALF = 18 * 128, EACH = 5, SLOTS = EACH * NTHR;
         static_assert(2 * HALF + 1 <= SLOTS && sizeof(uint32_t) * SLOTS <= sizeof(queue), "slots");
         uint32_t *count = (uint32_t *)&queue[0][0];
@@ -281,7 +437,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             return i < (uint32_t)HALF ? (int)(h & 0x8000u ? HALF + 1 + i : HALF - 1 - i) : -1;
         };
         auto value_at = [&](int r) { return __uint_as_float((r < HALF ? 0x3b00u + (HALF - 1 - r) : 0xbb00u + (r - HALF - 1)) << 16); };
-        if (!s.greedy && (s.p < 1.0 || (s.k > 0 && s.k < V)) && !short_list) {
+        if (!s.greedy && (ranks || s.p < 1.0) && !short_list) {
             for (int r = tid; r < SLOTS; r += NTHR) count[r] = 0;
             if (tid == 0) { listed = 0; at_found = 0; found[0] = SLOTS; found[1] = SLOTS; found[2] = 0; }
             __syncthreads();
@@ -320,7 +476,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             fits = fits && top > -INFINITY && (!(at_found & 1) || ((double)top + 512.0) * s.c > 42.0) && !(s.minw > 1099511627776.0);
             if (fits) {
                 m = top;
-                md = (double)m;
+                weigh.set(m, s.c);
                 u64 w[EACH], sum = 0, total, near_sum;
                 bool light[EACH];                      // min-p drops the slot
                 u64 near_mine = 0;
@@ -339,7 +495,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
                 }
                 bool mixed = n_near > 0 && heavies > 0 && heavies < (u64)n_near;      // a cut between the listed ones
                 int c_slot = SLOTS, c_ties = 0;        // kept: slots before c_slot, and c_ties logits of it
-                if (s.k > 0 && s.k < V) {
+                if (ranks) {
                     u64 n = 0, all;
 #pragma unroll
                     for (int q = 0; q < EACH; ++q) n += cnt[q];
@@ -445,8 +601,12 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     }
     float mine = -INFINITY;                            // this lane's largest logit (the maximum passes NaN over)
     if (!done) {
-        each8([&](int, const f8 &v) { mine = fmaxf(mine, max8(v)); });
-        mine = clean(mine);
+        if constexpr (SPLIT) {
+            for (int g = tid; g < groups; g += NTHR) mine = fmaxf(mine, ws_row.top[g]);
+        } else {
+            each8([&](int, const f8 &v) { mine = fmaxf(mine, max8(v)); });
+            mine = clean(mine);
+        }
         m = team_max<64>(mine);
         __syncthreads();
         if (lane == 0) wf[wave] = m;
@@ -455,6 +615,17 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         for (int w = 0; w < NW; ++w) m = fmaxf(m, wf[w]);
         if (m == -INFINITY) { if (tid == 0) a.out[row] = -1; return; }
         if (s.greedy) {
+            if constexpr (SPLIT) {
+                for (int g = tid; g < groups; g += NTHR) if (ws_row.top[g] == m) { atomicMin(&at_found, g); break; }
+                __syncthreads();
+                if (wave == 0) {
+                    const int c = at_found * SMP_GROUP + lane * 2;
+                    const uint64_t even = __ballot(c < V && (float)l[c < V ? c : V - 1] == m), odd = __ballot(c + 1 < V && (float)l[c + 1 < V ? c + 1 : V - 1] == m);
+                    const int i0 = even ? 2 * (__ffsll((long long)even) - 1) : SMP_GROUP, i1 = odd ? 2 * __ffsll((long long)odd) - 1 : SMP_GROUP;
+                    if (lane == 0) a.out[row] = at_found * SMP_GROUP + (i0 < i1 ? i0 : i1);
+                }
+                return;
+            }
             if (mine == m) {
                 int first = 0x7fffffff;
                 each8([&](int c, const f8 &v) {
@@ -467,45 +638,44 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
             if (tid == 0) a.out[row] = at_found;
             return;
         }
-        inf = m == INFINITY;
-        md = inf ? 0.0 : (double)m;
+        weigh.set(m, s.c);
     }
     // ---- top-k on a short list ---------------------------------------------------------------------------------------
     if (!done && short_list) {
         // A bound that k of the lanes' maxima reach, and not many more: the ordered bits of the maximum less a power of two (2^23 is an
-        // octave), eight powers at a time; then, if that leaves too many, the k-th largest's upper bits, two at a time.
+        // octave), eight powers at a time; then, while that leaves too many, the ninth of the range that holds the k-th largest
+        // (bounds that left up to 2 k + 256 made the list's sorting the longest step: 32 rows of 16384, k = 50, 25 us; now 13).
         const uint32_t key = ordered(mine), top_key = ordered(m);
-        uint32_t low = 0;
-        int reach = 0;
-        for (int b = 18; b < 32 && reach < s.k; b += 8) {
-            int *buf = wi[(b >> 3) & 1];
+        uint32_t low = 0, high = top_key;              // at least k reach low, fewer than k reach high (but where low is high)
+        int reach = 0, turn = 0;
+        auto eight = [&](auto bound) {                 // the first of bound(0 .. 7) that k reach, 8 if none; their number in `reach`
+            int *buf = wi[turn++ & 1];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                const uint32_t want = b + q < 32 && top_key > 1u << (b + q) ? top_key - (1u << (b + q)) : 0;
-                const int c = __popcll(__ballot(key >= want));
+                const int c = __popcll(__ballot(key >= bound(q)));
                 if (lane == 0) buf[q * NW + wave] = c;
             }
             __syncthreads();
-            for (int q = 0; q < 8 && reach < s.k; ++q) {
-                reach = 0;
+            for (int q = 0; q < 8; ++q) {
+                int n = 0;
 #pragma unroll
-                for (int w = 0; w < NW; ++w) reach += buf[q * NW + w];
-                low = b + q < 32 && top_key > 1u << (b + q) ? top_key - (1u << (b + q)) : 0;
+                for (int w = 0; w < NW; ++w) n += buf[q * NW + w];
+                if (n >= s.k) { reach = n; return q; }
             }
+            return 8;
+        };
+        for (int b = 18; b < 32 && reach == 0; b += 8) {
+            auto below = [&](int q) { return b + q >= 0 && b + q < 32 && top_key > 1u << (b + q) ? top_key - (1u << (b + q)) : 0u; };
+            const int q = eight(below);
+            if (q > 0) high = below(q - 1);
+            if (q < 8) low = below(q);
         }
-        if (reach > 2 * s.k + 256) {
-            low = 0;
-            __syncthreads();
-            for (int b = 30; b >= 12; b -= 2) {
-                int *buf = wi[(b >> 1) & 1];
-                const int c1 = __popcll(__ballot(key >= (low | 1u << b))), c2 = __popcll(__ballot(key >= (low | 2u << b))), c3 = __popcll(__ballot(key >= (low | 3u << b)));
-                if (lane == 0) { buf[wave] = c1; buf[NW + wave] = c2; buf[2 * NW + wave] = c3; }
-                __syncthreads();
-                int n1 = 0, n2 = 0, n3 = 0;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) { n1 += buf[w]; n2 += buf[NW + w]; n3 += buf[2 * NW + w]; }
-                low |= (n3 >= s.k ? 3u : n2 >= s.k ? 2u : n1 >= s.k ? 1u : 0u) << b;
-            }
+        while (reach > s.k + s.k / 4 + 16 && high - low > 1) {
+            const uint32_t step = (high - low) / 9 > 0 ? (high - low) / 9 : 1, was = low, up = high;
+            auto even = [&](int q) { const uint32_t x = was + (8 - q) * step; return x < up ? x : up; };
+            const int q = eight(even);
+            if (q > 0) high = even(q - 1);
+            if (q < 8) low = even(q);
         }
         // as a logit (what lies between -0 and +0 becomes 0, a key below every logit's becomes -inf)
         float from = low <= 0x007fffffu ? -INFINITY : value_of((u64)low << 32);
@@ -555,8 +725,8 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         }
     }
     // ---- any cut -----------------------------------------------------------------------------------------------------
-    const float per_step = fminf((float)(s.c * 0.69314718055994531 * (double)(SMP_BINS / SMP_RANGE)), 1e30f);
-    auto step_of = [&](float x) { return inf ? (x == m ? 0.f : SMP_BINS - 1.f) : fminf((m - x) * per_step, SMP_BINS - 1.f); };      // never falls as x falls; the step is its whole part
+    const float per_step = weigh.per_step;
+    auto step_of = [&](float x) { return weigh.step(x); };
     auto clear = [&]() {
         __syncthreads();
         for (int b = tid; b < SMP_BINS; b += NTHR) hist[b] = 0;
@@ -582,6 +752,10 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // cut where the sum of wt over the elements that `was` keeps reaches its goal
     auto find_cut = [&](const Cut &was, bool counts, auto wt, auto goal) {
         const bool any = was.x == -INFINITY;
+        if (SPLIT && !ranks) {                         // sample_weights_kernel has made it
+            __syncthreads();
+            for (int b = tid; b < SMP_BINS; b += NTHR) hist[b] = ws_row.hist[b];
+        } else {
         clear();
         each8([&](int i0, const f8 &v) {
 #pragma unroll
@@ -591,6 +765,7 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
                 if ((counts ? v[e] > -INFINITY : q < SMP_BINS - 1.f) && (any || inside(was, v[e], i0 + e))) atomicAdd(&hist[(int)q], w);
             }
         });
+        }
         u64 want = scan(goal);
         if (found[0] == SMP_BINS) return was;          // the goal is not reached: all are kept
         const int step = (int)found[0];
@@ -660,23 +835,10 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
         return c;
     };
     if (!done) {
-    if (s.k > 0 && s.k < V) cut = find_cut(cut, true, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
+    if (ranks) cut = find_cut(cut, true, [](float) -> u64 { return 1; }, [&](u64) { return (u64)s.k; });
     if (s.p < 1.0) cut = find_cut(cut, false, weight, [&](u64 total) { return goal_of(s.p, total); });
-    // min-p is a cut too: the smallest logit that weighs enough, by halving the ordered bit patterns up to the maximum's
     if (s.minw > 0.0) {
-        uint32_t lo = 0x007fffffu, hi = ordered(m);    // lo: -inf, too light; hi: weighs enough, or is the largest anyway
-        auto enough = [&](uint32_t key) { return weight_raw(value_of((u64)key << 32)) >= s.minw; };
-        const uint32_t near = ordered(clean((float)(md + (log2(s.minw) - SMP_BITS) / s.c)));       // almost always within two patterns
-        if (near > lo + 2 && near + 2 < hi) {
-            if (enough(near + 2)) hi = near + 2;
-            if (!enough(near - 2)) lo = near - 2;
-        }
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (enough(mid)) hi = mid;
-            else lo = mid;
-        }
-        const float x = value_of((u64)hi << 32);
+        const float x = weigh.min_p_cut(s.minw);
         int at = 0x7fffffff;
         if (s.minw > 1099511627776.0) {                // nothing weighs enough: the largest logit's lowest index stays
             if (tid == 0) at_found = 0x7fffffff;
@@ -696,7 +858,8 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
     // 64 lanes weigh 64 kept logits.
     const bool all = cut.x == -INFINITY;
     float *q = queue[wave];
-    each8([&](int i0, const f8 &v) {
+    if (SPLIT && !ranks && !(s.p < 1.0) && !(s.minw > 1099511627776.0)) for (int i = tid; i < pieces; i += NTHR) piece[i] = ws_row.piece[i];
+    else each8([&](int i0, const f8 &v) {
         u64 sum = 0;
         if (all) {
 #pragma unroll
@@ -759,25 +922,47 @@ __global__ __launch_bounds__(NTHR) void sample_row_kernel(const SampleArgs a) {
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 namespace {
+// Few long rows: maxima and weights are taken by many workgroups, one or two launches more.  In us, one workgroup per row and this, bf16
+// rows of 128000: 1 row without a cut 41 and 17, with min-p 35 and 17, k = 50 21 and 15; 64 rows 43 and 25, 37 and 29, 23 and
+// 17; 128 rows with min-p 38 and 45.  1 row of 65536 without a cut 24 and 16, of 40000 16 and 17.  Top-p alone: fp32 98 and 58,
+// bf16, whose values are counted, 53 and 64.  Where the largest logit's index is all that is asked for: 10 and 14.
+bool split_rows(const dnag_sample_args &p) {
+    if (p.vocab < 65536 || p.vocab > SMP_MAX_V || p.rows < 1 || p.rows > 64 || p.top_k_rows || !(p.temperature_rows || p.temperature > 0.0)) return false;
+    if (p.top_k > 0 && p.top_k < p.vocab) return p.top_k <= short_list_k(p.vocab, p.dtype == DNAG_BF16);
+    return p.dtype != DNAG_BF16 || !(p.top_p_rows || p.top_p < 1.0);
+}
+int64_t space_of_row(int64_t V) { return (SMP_BINS * 8 + ws_pieces(V) * 8 + ws_groups(V) * 4 + 255) / 256 * 256; }
+
+template <class T, bool SPLIT>
+int launch_long(const SampleArgs &a, hipStream_t st) {
+    const size_t bytes = (size_t)ws_pieces(a.V) * 8 + (__is_same(T, tbf16) ? 5120 * 8 : 0);      // pieces, and the slots' weights
+    static LdsLimit limit;
+    if (int rc = limit.allow((const void *)sample_row_kernel<T, 1024, SPLIT>, bytes + 65536)) return rc;      // beside 50 KB that are static
+    hipLaunchKernelGGL((sample_row_kernel<T, 1024, SPLIT>), dim3((unsigned)a.rows), dim3(1024), bytes, st, a);
+    return 0;
+}
 template <class T>
 int launch(const SampleArgs &a, hipStream_t st) {
     if (a.V <= 64) {
         const int G = pow2_at_least(a.V, 2, 64);
         hipLaunchKernelGGL((sample_small_kernel<T>), dim3((unsigned)ceil_div(a.rows, 256 / G)), dim3(256), 0, st, a, G);
     } else if (a.V <= 4096) {
-        hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), (size_t)ceil_div(a.V, 512) * 8, st, a);
-    } else {
-        const size_t bytes = (size_t)ceil_div(a.V, 512) * 8 + (__is_same(T, tbf16) ? 5120 * 8 : 0);      // pieces, and the slots' weights
-        static LdsLimit limit;
-        if (int rc = limit.allow((const void *)sample_row_kernel<T, 1024>, bytes + 65536)) return rc;      // beside 50 KB that are static
-        hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), bytes, st, a);
-    }
+        hipLaunchKernelGGL((sample_row_kernel<T, 256, false>), dim3((unsigned)a.rows), dim3(256), (size_t)ws_pieces(a.V) * 8, st, a);
+    } else if (a.ws) {
+        hipLaunchKernelGGL((sample_groups_kernel<T>), dim3((unsigned)ceil_div(a.V, 2048), (unsigned)a.rows), dim3(256), 0, st, a);
+        if (!(a.top_k1 > 0 && a.top_k1 < a.V)) hipLaunchKernelGGL((sample_weights_kernel<T>), dim3((unsigned)ceil_div(a.V, 4096), (unsigned)a.rows), dim3(256), 0, st, a);
+        if (int rc = launch_long<T, true>(a, st)) return rc;
+    } else if (int rc = launch_long<T, false>(a, st)) return rc;
     TOK_TRY(hipGetLastError());
     return 0;
 }
 }  // namespace
 
 extern "C" size_t dnag_sample_args_bytes(void) { return sizeof(dnag_sample_args); }
+
+extern "C" size_t dnag_sample_workspace_bytes(const dnag_sample_args *p) {
+    return p && split_rows(*p) ? (size_t)(p->rows * space_of_row(p->vocab)) : 0;
+}
 
 extern "C" int dnag_sample_tokens(const dnag_sample_args *p) {
     if (!p) return dnag_fail(DNAG_E_ARG, "NULL pointer");
@@ -792,6 +977,11 @@ extern "C" int dnag_sample_tokens(const dnag_sample_args *p) {
     a.u = p->u; a.temperature = p->temperature_rows; a.top_p = p->top_p_rows; a.min_p = p->min_p_rows; a.top_k = p->top_k_rows;
     a.temperature1 = p->temperature; a.top_p1 = p->top_p; a.min_p1 = p->min_p; a.top_k1 = p->top_k;
     a.out = p->out;
+    if (const size_t need = dnag_sample_workspace_bytes(p)) {
+        if (!p->workspace || p->workspace_bytes < need) return dnag_fail(DNAG_E_WORKSPACE, "workspace has %zu bytes, %zu are needed", p->workspace_bytes, need);
+        a.ws = (char *)p->workspace;
+        a.ws_row = space_of_row(a.V);
+    }
     hipStream_t st = (hipStream_t)p->stream;
     return p->dtype == DNAG_F32 ? launch<float>(a, st) : p->dtype == DNAG_BF16 ? launch<tbf16>(a, st) : launch<tf16>(a, st);
 }

@@ -505,6 +505,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[N
     n, V = lg.shape
     if n:
         t, k, p, q = numbers
-        _launch_args(_lib.load().dnag_sample_tokens, index, "dnag_sample_tokens", _lib.SAMPLE_LAYOUT, n, V, stride, code, max(-1, min(int(k), 0x7fffffff)), t, p, q,
-                     lg.data_ptr(), uc.data_ptr(), *map(_p, rows), out.data_ptr())
+        lib = _lib.load()
+        fields = (n, V, stride, code, max(-1, min(int(k), 0x7fffffff)), t, p, q, lg.data_ptr(), uc.data_ptr(), *map(_p, rows), out.data_ptr())
+        nbytes = lib.dnag_sample_workspace_bytes(_lib.SAMPLE_LAYOUT.pack(*fields, 0, 0, 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+        _launch_args(lib.dnag_sample_tokens, index, "dnag_sample_tokens", _lib.SAMPLE_LAYOUT, *fields, _p(ws), nbytes)
     return out

@@ -485,9 +485,12 @@ typedef struct dnag_sample_args {
     const int32_t *top_k_rows;
     const float *top_p_rows, *min_p_rows;
     int64_t *out;
+    void *workspace;                                       /* dnag_sample_workspace_bytes; NULL where that is 0 */
+    size_t workspace_bytes;
     void *stream;
 } dnag_sample_args;
 size_t dnag_sample_args_bytes(void);
+size_t dnag_sample_workspace_bytes(const dnag_sample_args *args);
 int dnag_sample_tokens(const dnag_sample_args *args);
 
 /* ---- kernel timing for bench.py ----------------------------------------------------------------

@@ -6,11 +6,13 @@ operations (products, the levels of a sum over a row, a reciprocal root) by CHAI
 CHAIN = 64: a row sum is 8 + 10 + 16 levels (lane, wave, workgroup), twice for LayerNorm, and there are fewer than 16 other
 operations in any chain.  A sum over n rows adds n 2^-24 of its magnitudes (the worst order)."""
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
 
-from diffusionnag_amd import arch_functions as AF, ema as ema_lib, losses, token_ops as ops, utils
+from diffusionnag_amd import arch_functions as AF, ema as ema_lib, losses, run_lib, token_ops as ops, utils
 from tests import token_reference as R
 from tests.helpers import Cfg
 from tests.token_reference import U32, half_step
@@ -407,7 +409,7 @@ def want_tokens(x, u, temperature, top_k, top_p, min_p):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,V", [(1, 1), (50, 2), (300, 7), (300, 9), (70, 33), (40, 64), (40, 65), (30, 511), (20, 4096), (12, 4097), (6, 20001), (2, 140000)])
+@pytest.mark.parametrize("rows,V", [(1, 1), (50, 2), (300, 7), (300, 9), (70, 33), (40, 64), (40, 65), (30, 511), (20, 4096), (12, 4097), (6, 20001), (66, 16500), (2, 140000)])
 def test_sample_tokens(dtype, rows, V):
     g = gen(rows * V)
     x = rnd(g, rows, V, dtype=dtype, std=2.5)
@@ -428,7 +430,7 @@ def test_sample_tokens(dtype, rows, V):
         assert got.dtype == torch.int64 and got.cpu().tolist() == want_tokens(x, u, **full), f"{settings}"
 
 
-@pytest.mark.parametrize("V", [7, 64, 100, 4500])
+@pytest.mark.parametrize("V", [7, 64, 100, 4500, 66000])
 def test_sample_ties_and_extremes(V):
     g = gen(V)
     u = torch.rand(24, generator=g)
@@ -462,11 +464,12 @@ def test_sample_ties_and_extremes(V):
 
 
 @pytest.mark.parametrize("what", ["normal", "near 0", "far", "halves", "few values", "masked low", "one"])
-def test_sample_bf16_values(what):
+@pytest.mark.parametrize("V", [9001, 65541])
+def test_sample_bf16_values(what, V):
     """Rows that the counting of bf16 values meets: spread ones, many within 2^-9 of 0 (more than its list holds, too), beyond 2^9, ties at
     every cut, masked with large negative numbers."""
     g = gen(len(what))
-    rows, V = 6, 9001
+    rows = 6
     x = rnd(g, rows, V, std=2.5)
     if what == "near 0":
         x = x * torch.tensor([1e-4, 1e-3, 4e-3, 0.02, 0.1, 0.3])[:, None]
@@ -490,6 +493,28 @@ def test_sample_bf16_values(what):
                      dict(top_k=1500, top_p=0.999, min_p=1e-4), dict(min_p=1.0), dict(temperature=30.0, top_p=0.7)):
         full = {**dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **settings}
         assert ops.sample_tokens(dev(x), dev(u), **settings).cpu().tolist() == want_tokens(x, u, **full), f"{settings}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_few_rows_as_many(dtype):
+    """Few long rows are shared by many workgroups: the same tokens as among more rows than that, also where a cut by rank meets rows with
+    less than k logits, and top-k alone where each group of logits has at most a few of the largest."""
+    g = gen(5)
+    rows, V = 96, 70001
+    x = rnd(g, rows, V, dtype=dtype, std=2.5)
+    x[1, 40:] = -float("inf")
+    x[2] = torch.round(x[2])
+    x[3] = x[3].sort(descending=True).values           # the largest side by side
+    x[4] = -float("inf")
+    x[5, V - 1] = 40.0
+    x, u = dev(x), dev(torch.rand(rows, generator=g))
+    many = dict(temperature=torch.rand(rows, generator=g) + 0.2, top_k=torch.randint(0, 40, (rows,), generator=g, dtype=torch.int32) ** 2, top_p=torch.rand(rows, generator=g) + 0.3)
+    many = {k: dev(v) for k, v in many.items()}
+    many["temperature"][6] = 0.0
+    for settings in (dict(), dict(temperature=0.0), dict(min_p=0.05), dict(min_p=3.0), dict(top_k=1), dict(top_k=60), dict(top_k=60, temperature=many["temperature"]), dict(top_k=200, top_p=0.9), dict(top_k=900), dict(top_k=5000, min_p=0.01),
+                     dict(top_p=0.9), dict(top_p=0.3, min_p=0.1), dict(temperature=20.0, top_p=0.99), many):
+        some = {k: v[:9] if torch.is_tensor(v) else v for k, v in settings.items()}
+        assert torch.equal(ops.sample_tokens(x[:9], u[:9], **some), ops.sample_tokens(x, u, **settings)[:9]), f"{settings}"
 
 
 def test_sample_frequencies():
@@ -517,6 +542,32 @@ def test_drawing_ends_a_sampling_round():
     assert int(counts[0]) == 64 and (status == -1).all()
     want = R.sample_row(x[5, 3].numpy(), float(u[5, 3]), 0.5, 0, 1.0, 0.0)
     assert int(one[5, 3].argmax()) == want
+
+
+def test_generate_archs_meta_draws():
+    """``args.draw_temperature`` ends a round by drawing; without it the sampler's output is thresholded as before."""
+    g = gen(3)
+    x = torch.rand(32, 8, 7, generator=g)
+    x[:, 0, 0] += 20
+    x[:, 7, 1] += 20
+    x[:, 1:7, :2] = -float("inf")
+    sampling_fn = lambda *a, **kw: dev(x)                                                                # noqa: E731
+    config, model = SimpleNamespace(device=DEV), torch.nn.Identity()
+    run = lambda **kw: run_lib.generate_archs_meta(config, sampling_fn, model, None, model, 32, patient_factor=1,    # noqa: E731
+                                                   args=SimpleNamespace(classifier_scale=1.0, scale_step=0.1, **kw))
+
+    def first_seen(sample):
+        seen = AF.new_seen_table(DEV)
+        AF.device_validity(sample, seen, 0)
+        first = seen.cpu()
+        codes = (first != AF.UNSEEN).nonzero()[:, 0]
+        return [AF.code_to_string(int(c)) for c in codes[first[codes].sort(stable=True).indices]]
+    torch.manual_seed(9)
+    got = run(draw_temperature=0.7, draw_top_p=0.9, draw_min_p=0.05)
+    torch.manual_seed(9)
+    u = torch.rand(32, 8, device=DEV)
+    assert got == first_seen(utils.draw_onehot(dev(x), u, temperature=0.7, top_p=0.9, min_p=0.05)) and len(got) > 1
+    assert run() == run(draw_temperature=0.0) == first_seen(dev(x))
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -196,6 +196,13 @@ def test_c_entries_check_before_they_launch():
                       (dict(logits_stride=7), "stride"), (dict(u=None), "NULL"), (dict(out=None), "NULL")):
         refused(lib.dnag_sample_tokens(C.byref(sample(**kw))), words)
     assert lib.dnag_sample_tokens(C.byref(sample(rows=0))) == 0
+    few = sample(rows=2, vocab=70000, logits_stride=70000)
+    need = lib.dnag_sample_workspace_bytes(C.byref(few))
+    assert need >= 2 * 70000 // 128 * 4
+    for kw in (dict(workspace=None, workspace_bytes=need), dict(workspace=P, workspace_bytes=need - 1)):
+        refused(lib.dnag_sample_tokens(C.byref(sample(rows=2, vocab=70000, logits_stride=70000, **kw))), "workspace")
+    for kw in (dict(rows=500), dict(rows=-1), dict(rows=1 << 40), dict(vocab=1 << 21), dict(temperature=0.0), dict(top_k_rows=P), dict(top_k=5000)):
+        assert lib.dnag_sample_workspace_bytes(C.byref(sample(**{**dict(rows=2, vocab=70000, logits_stride=70000), **kw}))) == 0
 
 
 def test_eager_graph_of_the_same_leaf_is_noticed(monkeypatch):
