@@ -8,8 +8,8 @@
 // above 131072 16-bit or 65536 fp32 logits (NV = 0) the row is read again, out of the caches.  The teacher's entries are the first wave's work beside
 // that; the few elements of the gradient that hold an entry are written again, in full precision, behind the row.
 // Sums are fp32, in a fixed order.  Exponentials are v_exp_f32 (1 ulp) of s c - R, one fused operation, with c = log2(e) / tau and R the
-// rounded c max(s): R is a reference that divides out, so its rounding does not matter.
-// 8192 x 32000 bf16, loss and gradient: 242 us, 4.3 TB/s.  1000 x 50001 fp16, loss: 34 us, 3.0 TB/s: rows of odd length are read by
+// rounded c max(s): what its rounding takes from every exponent is one factor, taken out of the sum.
+// 8192 x 32000 bf16, loss and gradient: 245 us, 4.3 TB/s.  1000 x 50001 fp16, loss: 34 us, 3.0 TB/s: rows of odd length are read by
 // 2-byte-aligned vector loads and the chip runs 1000 workgroups on 256 CUs, a few each.
 #include "dnag_token_common.h"
 #include <math.h>
@@ -25,7 +25,7 @@ struct DistillArgs {
     const float *wsum;                                 // sum of the positive weights (mean with weights) or NULL
     float scale;                                       // 1 / rows (mean without weights) or 1
     float *row_loss;                                   // [rows] or NULL: w_t tau^2 KL_t
-    float *stats;                                      // [rows][2] or NULL: reference R, sum of exponentials
+    float *stats;                                      // [rows][2] or NULL: largest logit, sum of exponentials relative to it
     const float *gout;                                 // MODE 2: upstream gradient, gout[t * gstep]
     int64_t gstep;
     void *grad;
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
 (const DistillArgs a) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1, TW = TPR < 64 ? TPR : 64;      // TW: lanes that handle the teacher's entries
     constexpr int NR = NV > 0 ? NV : 1;
-    constexpr float LOW = -3.0e38f;                    // below every logit that counts: -inf - LOW = -inf, exp2 = 0
+    constexpr float LOW = __is_same(T, tf16) ? -65536.f : -3.402823466e38f;      // no finite logit is below: -inf - LOW = -inf, exp2 = 0
     typedef typename Vec8<T>::type raw8;
     extern __shared__ char lds[];
     __shared__ float red[33];                          // pairs of the waves; [32]: the teacher's maximum
@@ -105,35 +105,43 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
     constexpr bool KEEP = MODE == 1 && NV > 0 && NV <= 8;      // 16 pieces: their registers would spill
     float ref, sum, tr = LOW, own = 0.f;
     f8 ex[KEEP ? NV : 1];
-    auto exps = [&](f8 v, float r) {
+    // exp((x - r) / tau) times 2^(r c - R) for R the rounded r c, a power near 1 that `true_to` takes out; where the reference is so large that
+    // it is not near 1 (a mask's values all over a row), from the difference
+    // (fp16 cannot get there from a temperature of 0.1 on, the least that is built for it: the difference and its registers cost the loss of
+    // 1000 x 50001 38 us for 32)
+    auto far = [&](float r) { return __is_same(T, tf16) ? false : !(fabsf(r * a.c2) < 1048576.f); };
+    auto exps = [&](f8 v, float r) {                   // (without a branch: two forms of it took 6 % longer)
+        const float base = far(r) ? r : 0.f, R = far(r) ? 0.f : r * a.c2;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = exp2_hw(fmaf(v[e], a.c2, -r));
+        for (int e = 0; e < 8; ++e) v[e] = exp2_hw(fmaf(v[e] - base, a.c2, -R));
         return v;
     };
+    auto true_to = [&](float r) { return far(r) ? 1.f : exp2_hw(-fmaf(r, a.c2, -(r * a.c2))); };
+    auto shift = [&](float from, float to) { return exp2_hw((from - to) * a.c2); };
     if constexpr (MODE == 2) { ref = a.stats[2 * row]; sum = a.stats[2 * row + 1]; }
     else {
         if constexpr (NV > 0) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) tr = fmaxf(tr, max8(widen<T>(x[j])));
-            tr = fmaxf(tr * a.c2, LOW);                // (a lane without logits: LOW)
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const f8 v = exps(widen<T>(x[j]), tr);
                 own += sum8(v);
                 if constexpr (KEEP) ex[j] = v;
             }
+            own *= true_to(tr);
         } else
             for (int c = lane * 8; c < a.V; c += tpr * 8) {
                 const f8 v = load8_n(s + c, a.V - c, -INFINITY);
-                const float nr = fmaxf(tr, max8(v) * a.c2);
-                own *= exp2_hw(tr - nr);
+                const float nr = fmaxf(tr, max8(v));
+                own *= shift(tr, nr);
                 tr = nr;
-                own += sum8(exps(v, tr));
+                own += sum8(exps(v, tr)) * true_to(tr);
             }
         ref = tr;
 #pragma unroll
         for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
-        sum = own * exp2_hw(tr - ref);
+        sum = own * shift(tr, ref);
 #pragma unroll
         for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if constexpr (TPR > 64) {
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
             const int waves = tpr >> 6;
             for (int w = 0; w < waves; ++w) ref = fmaxf(ref, red[2 * w]);
             sum = 0.f;
-            for (int w = 0; w < waves; ++w) sum += red[2 * w + 1] * exp2_hw(red[2 * w] - ref);
+            for (int w = 0; w < waves; ++w) sum += red[2 * w + 1] * shift(red[2 * w], ref);
         }
     }
     if constexpr (MODE < 2) {
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
             for (int k = lane; k < a.K; k += TW) {
                 if (ti[k] < 0) continue;
                 const float u = (tp[k] - tmax) * a.c2, p = exp2_hw(u) / tsum;
-                if (!(p == 0.f)) l += p * ((u - ltsum) - (fmaf(ts[k], a.c2, -ref) - lsum));
+                if (!(p == 0.f)) l += p * ((u - ltsum) - ((ts[k] - ref) * a.c2 - lsum));
             }
 #pragma unroll
             for (int o = TW / 2; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
@@ -167,8 +175,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
         if (a.wsum) f /= *a.wsum;                      // positive: this row's weight is part of it
         if constexpr (MODE == 2) f *= a.gout[row * a.gstep];
         const float fq = f / sum;
+        const float ft = fq * (KEEP ? true_to(tr) * shift(tr, ref) : true_to(ref));
         if constexpr (KEEP) {
-            const float ft = fq * exp2_hw(tr - ref);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * tpr + lane) * 8;
@@ -178,10 +186,10 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * tpr + lane) * 8;
-                if (c < a.V) store8_n(g + c, exps(widen<T>(x[j]), ref) * fq, a.V - c);
+                if (c < a.V) store8_n(g + c, exps(widen<T>(x[j]), ref) * ft, a.V - c);
             }
         } else
-            for (int c = lane * 8; c < a.V; c += tpr * 8) store8_n(g + c, exps(load8_n(s + c, a.V - c), ref) * fq, a.V - c);
+            for (int c = lane * 8; c < a.V; c += tpr * 8) store8_n(g + c, exps(load8_n(s + c, a.V - c), ref) * ft, a.V - c);
         if constexpr (TPR > 64) __syncthreads();       // the row is written before its entries are
         else wave_fence();
         if (lane < TW)
@@ -192,7 +200,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void distill_kernel
                 bool first = true;
                 for (int j = 0; j < a.K; ++j)
                     if (ti[j] == i) { z += exp2_hw((tp[j] - tmax) * a.c2); first &= j >= k; }
-                if (first) g[i] = (T)(f * (exp2_hw(fmaf(ts[k], a.c2, -ref)) / sum - z / tsum));
+                if (first) g[i] = (T)(f * (shift(ts[k], ref) / sum - z / tsum));
             }
     }
 }
@@ -247,7 +255,8 @@ int check(const dnag_distill_args *p) {
     if (p->rows < 0 || p->rows > 0x7fffffffll) return dnag_fail(DNAG_E_ARG, "rows=%lld out of range", (long long)p->rows);
     if (p->vocab < 1 || p->vocab > (1 << 30)) return dnag_fail(DNAG_E_ARG, "vocab=%lld out of range (1 .. 2^30)", (long long)p->vocab);
     if (p->k < 1 || p->k > DISTILL_MAX_K) return dnag_fail(DNAG_E_ARG, "k=%d out of range (1 .. %d)", p->k, DISTILL_MAX_K);
-    if (!(p->temperature > 0.f) || !(p->temperature < INFINITY)) return dnag_fail(DNAG_E_ARG, "temperature=%g must be positive and finite", (double)p->temperature);
+    const float least = p->dtype == DNAG_F16 ? 0.1f : 1e-6f;
+    if (!(p->temperature >= least && p->temperature <= 1e6f)) return dnag_fail(DNAG_E_ARG, "temperature=%g out of range (%g .. 1e6)", (double)p->temperature, (double)least);
     if (p->logits_stride < p->vocab) return dnag_fail(DNAG_E_ARG, "the logits' row stride %lld is smaller than vocab %lld", (long long)p->logits_stride, (long long)p->vocab);
     if (p->reduction < DNAG_REDUCE_NONE || p->reduction > DNAG_REDUCE_MEAN) return dnag_fail(DNAG_E_ARG, "unknown reduction %d", p->reduction);
     return 0;

@@ -54,7 +54,7 @@ __device__ __forceinline__ RowSet row_set(const SampleArgs &a, int64_t row) {
     RowSet s;
     const double t = a.temperature ? (double)a.temperature[row] : a.temperature1;
     s.greedy = !(t > 0.0);
-    s.c = 1.4426950408889634074 / t;
+    s.c = fmin(1.4426950408889634074 / t, 1e300);      // finite: the largest logit's distance of 0 times it is 0
     s.p = a.top_p ? (double)a.top_p[row] : a.top_p1;
     const double q = a.min_p ? (double)a.min_p[row] : a.min_p1;
     s.minw = q == q ? q * 1099511627776.0 : 0.0;

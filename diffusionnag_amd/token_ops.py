@@ -386,8 +386,9 @@ class _Distill:
             raise ValueError(f"k={teacher_ids.shape[-1]} teacher entries; 1 to 1024 are built")
         if reduction not in _REDUCE:
             raise ValueError(f"reduction={reduction!r}: 'none', 'sum' and 'mean' are built")
-        if not 0 < temperature < float("inf"):
-            raise ValueError(f"temperature={temperature} must be positive and finite")
+        least = 0.1 if logits.dtype == torch.float16 else 1e-6
+        if not least <= temperature <= 1e6:
+            raise ValueError(f"temperature={temperature} is outside {least} .. 1e6 ({logits.dtype} logits)")
         if teacher_ids.dtype not in _IDS:
             raise ValueError(f"teacher_ids have dtype {teacher_ids.dtype}; int32 and int64 are built")
         self.lead = logits.shape[:-1]
@@ -448,7 +449,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``teacher_ids`` [..., k] outside ``0 .. vocab - 1`` are no entries (a row shorter than k is filled with -1); repeated ids add up.
     ``row_weight`` [...] float32: rows whose weight is not positive (padding) count nothing and their logits do not
     matter, NaN included.  A row without entries counts 0.  ``reduction``: 'mean' over the positive weights (over all rows
-    without weights; 0 where there are none), 'sum', or 'none' (weighted loss of each row).  float32.  No gradient reaches the
+    without weights; 0 where there are none), 'sum', or 'none' (weighted loss of each row).  float32.  ``logits`` masked with -inf
+    or their type's lowest value have no probability (a row of nothing but lowest values: one and the same probability).
+    ``temperature`` is 1e-6 to 1e6 (float16 logits: from 0.1 on).  No gradient reaches the
     teacher or the weights: they must not require one."""
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
         raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")

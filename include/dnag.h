@@ -437,7 +437,8 @@ int dnag_block_norms_forward(const dnag_block_norms_args *args);
 int dnag_block_norms_grad(const dnag_block_norms_args *args);
 
 /* Distillation: KL divergence between the teacher's distribution over its `k` listed tokens and the student's over the whole
- * vocabulary, both at `temperature` (tau), times tau^2:  loss_t = w_t tau^2 sum_k p_k (log p_k - log q_{id_k}).
+ * vocabulary, both at `temperature` (tau), times tau^2:  loss_t = w_t tau^2 sum_k p_k (log p_k - log q_{id_k}),
+ * 1e-6 <= tau <= 1e6 (fp16 logits: from 0.1 on).
  * logits [rows][vocab] (row stride logits_stride) of type dtype; teacher_ids [rows][k] (ids_bytes 4 or 8; an id outside
  * 0 .. vocab - 1 is no entry, ids may repeat), teacher_logits [rows][k] of type teacher_dtype; row_weight fp32 [rows] or NULL.
  * A row without entries, or whose weight is not positive, counts 0 and its logits do not matter.

@@ -318,6 +318,7 @@ def distill_tolerances(logits, ids, tl, tau, w, reduction, grad):
     if reduction == "none":
         return row, None
     g = (weight * tau)[:, None] * (torch.softmax(z, 1) + torch.zeros_like(z).scatter_add_(1, ids.clamp(0, V - 1), torch.ones_like(tl).double())) * 2 * q / n
+    g = g + (weight * tau)[:, None] * 2.0 ** -126 / n  # an exponential below 2^-126 is 0 (v_exp_f32 gives no subnormal numbers)
     return row.sum() / n + len(w) * U32 * float((weight * tau * tau * span).sum()) / n, g
 
 
@@ -385,6 +386,37 @@ def test_distill_edges():
     full = torch.arange(11).expand(2, 3, 11)
     loss, grad = ops.distill_loss_and_grad(dev(s), dev(full), dev(s), reduction="none")
     assert loss.shape == (2, 3) and float(loss.abs().max()) <= 30 * (CHAIN + 3 * U32 * 90) and float(grad.abs().max()) <= 2 * (CHAIN + 3 * U32 * 90)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [7, 300, 5000, 60001, 140000])
+def test_distill_masks_of_the_lowest_value(dtype, V):
+    """Rows masked with their type's lowest value: in part, at temperatures that take its scaled value out of fp32, and whole (a padded
+    row without a weight: every token is as likely).  The exponents of masked tokens are exact (no weight at all, or 0 in the
+    whole row), so the tolerances are those of rows with -60 (or 0) in their place."""
+    g = gen(V)
+    rows, K = 4, 3
+    low = torch.finfo(dtype).min
+    x = rnd(g, rows, V, dtype=dtype, std=2.0)
+    x[0] = low
+    x[1, V // 2:] = low
+    x[2, 1:] = low
+    ids = torch.randint(0, max(1, V // 2), (rows, K), generator=g)
+    ids[2] = 0
+    x[3] += 30000 if dtype == torch.float16 else 1e7   # far from 0 as a whole, one step apart
+    tl = rnd(g, rows, K, dtype=dtype)
+    like = torch.where(x == low, -60.0, x.float())
+    like[0] = 0
+    like[3] -= like[3].max()                           # (exact differences)
+    for tau in (0.1, 0.6, 1.0, 1.5, 3.0):
+        want, grad = R.distill(x, ids, tl, tau, None, "sum")
+        tol, gtol = distill_tolerances(like, ids, tl, tau, torch.ones(rows), "sum", grad)
+        loss, got = ops.distill_loss_and_grad(dev(x), dev(ids), dev(tl), temperature=tau, reduction="sum")
+        within(loss, want, tol, f"loss, tau {tau}")
+        within(got, grad, gtol, f"gradient, tau {tau}")
+        leaf = dev(x).requires_grad_(True)
+        ops.distill_loss(leaf, dev(ids), dev(tl), temperature=tau, reduction="sum").backward()
+        within(leaf.grad, grad, gtol, f"gradient through autograd, tau {tau}")
 
 
 def test_distill_gradient_against_differences():
@@ -457,6 +489,8 @@ def test_sample_ties_and_extremes(V):
     assert ((got >= 0) & (got < V)).all()
     big = ops.sample_tokens(dev(two), dev(u), min_p=torch.full((24,), 2.0, device=DEV)).cpu().tolist()
     assert big == want_tokens(two, u, 1.0, 1, 1.0, 0.0)                # nothing is as likely as twice the largest: the largest stays
+    for t in (5e-324, 1e-308, 1e308):                                  # the ends of the temperature's range: the largest logit, or any
+        assert ops.sample_tokens(dev(wide), dev(u), temperature=t).cpu().tolist() == want_tokens(wide, u, t if t > 1 else 0.0, 0, 1.0, 0.0)
     strided = torch.full((24, V + 9), float("nan"))
     strided[:, 4:V + 4] = two
     assert torch.equal(ops.sample_tokens(dev(strided)[:, 4:V + 4], dev(u), top_p=0.6), ops.sample_tokens(dev(two), dev(u), top_p=0.6))

@@ -107,6 +107,8 @@ def test_cpu_tensors_are_refused():
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3), torch.zeros(2, 3)),
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=0.0),
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=float("inf")),
+    lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=1e-30),
+    lambda: ops.distill_loss(torch.zeros(2, 8).half(), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), temperature=0.09),
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), reduction="batchmean"),
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), row_weight=torch.zeros(3)),
     lambda: ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3), row_weight=torch.zeros(2).half()),
