@@ -93,6 +93,11 @@ def _p(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of the shape and type of ``t`` (empty_like takes half the time of empty: 1.1 and 2.2 us)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _leaf_mark(*tensors: Optional[torch.Tensor]) -> None:
     """Refuses to record a backward pass of leaves under graph capture while an eager graph of the same leaves is alive: their
     gradient accumulators belong to the eager graph's stream, and running them inside the capture ends the process."""
@@ -120,7 +125,7 @@ def _check_ids(ids: torch.Tensor) -> torch.Tensor:
 def _embed(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     index = _device(ids, weight)
     V, d = weight.shape
-    out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, d))
     n = ids.numel()
     if n:
         w, stride = _rows2d(weight)
@@ -176,7 +181,7 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
     index = _device(grad, ids)
     g, stride = _rows2d(grad)
     rows, d = g.shape
-    out = torch.empty((num_tokens, d), dtype=grad.dtype, device=grad.device)
+    out = grad.new_empty((num_tokens, d))
     nbytes = lib.dnag_embed_grad_workspace_bytes(rows, num_tokens, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
     _launch(lib.dnag_embed_grad, index, "dnag_embed_grad", ids.data_ptr(), _IDS[ids.dtype], rows, g.data_ptr(), stride, num_tokens, d, code, float(scale),
@@ -211,7 +216,7 @@ def _small(t: Optional[torch.Tensor], name: str, d: int, dtype) -> Optional[torc
 
 class _Seam:
     """The checked arguments of one ``block_norms`` call as the library takes them."""
-    __slots__ = ("index", "shape", "device", "dtype", "x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "rows", "d", "pre", "head",
+    __slots__ = ("index", "shape", "device", "dtype", "given_x", "given_y", "x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "rows", "d", "pre", "head",
                  "arrays")
 
     def __init__(self, x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype=None):
@@ -246,6 +251,7 @@ class _Seam:
         d = x.shape[-1]
         if d > 16384:
             raise ValueError(f"dim={d}: 1 to 16384 are built")
+        self.given_x, self.given_y = x, y
         self.x, xs = _rows2d(x)
         rows = self.x.shape[0]
         self.y, ys = (None, 0) if y is None else _rows2d(y)
@@ -274,12 +280,18 @@ class _Seam:
         self.arrays = (self.x.data_ptr(), _p(self.y), _p(gate), _p(self.post_weight), _p(self.post_bias), _p(self.pre_weight), _p(self.pre_bias), xs, ys)
 
     def forward(self):
-        x_new = torch.empty(self.shape, dtype=self.x.dtype, device=self.device) if self.y is not None else None
-        h = torch.empty(self.shape, dtype=self.dtype, device=self.device) if self.pre else None
+        x_new = _like(self.given_x) if self.y is not None else None
+        h = self._branch() if self.pre else None
         if self.rows:
             _launch_args(_lib.load().dnag_block_norms_forward, self.index, "dnag_block_norms_forward", _lib.BLOCK_NORMS_LAYOUT, *self.head, *self.arrays,
                          _p(x_new), _p(h), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         return x_new, h
+
+    def _branch(self) -> torch.Tensor:
+        """A new tensor of the branch's type."""
+        if self.given_y is not None:
+            return _like(self.given_y)
+        return _like(self.given_x) if self.dtype == self.x.dtype else torch.empty(self.shape, dtype=self.dtype, device=self.device)
 
     def backward(self, grad_x, grad_h, wanted) -> BlockNormsGrad:
         gxs = ghs = 0
@@ -295,10 +307,10 @@ class _Seam:
             grad_h, ghs = _rows2d(grad_h)
         _device(self.x, grad_x, grad_h)
         dev, rows = self.device, self.rows
-        new = torch.empty if rows else torch.zeros
-        dx = torch.empty(self.shape, dtype=self.x.dtype, device=dev)
-        dy = torch.empty(self.shape, dtype=self.dtype, device=dev) if self.y is not None else None
-        grads = [new(t.shape, dtype=t.dtype, device=dev) if t is not None and n in wanted else None for n, t in
+        new = torch.empty_like if rows else torch.zeros_like                              # (contiguous as they are kept)
+        dx = _like(self.given_x)
+        dy = self._branch() if self.y is not None else None
+        grads = [new(t) if t is not None and n in wanted else None for n, t in
                  zip(_SMALL, (self.gate, self.post_weight, self.post_bias, self.pre_weight, self.pre_bias))]
         if rows:
             lib = _lib.load()
@@ -396,6 +408,7 @@ class _Distill:
             raise ValueError(f"row_weight must be {tuple(self.lead)} float32, got {tuple(row_weight.shape)} {row_weight.dtype}")
         code, tcode = _dtype(logits, "logits"), _dtype(teacher_logits, "teacher_logits")
         self.index, self.device, self.reduction = _device(logits, teacher_ids, teacher_logits, row_weight), logits.device, reduction
+        self.given = logits
         self.logits, stride = _rows2d(logits)
         self.rows, self.V = self.logits.shape
         self.kept = (teacher_ids.contiguous(), teacher_logits.contiguous(), None if row_weight is None else row_weight.contiguous())
@@ -413,13 +426,13 @@ class _Distill:
         none = self.reduction == "none"
         loss = (torch.empty if self.rows else torch.zeros)(self.lead if none else (), dtype=torch.float32, device=self.device)
         st = torch.empty(self.rows, 2, dtype=torch.float32, device=self.device) if stats else None
-        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.device) if grad else None
+        g = _like(self.given) if grad else None
         if self.rows:
             self._call("dnag_distill_loss_grad" if grad else "dnag_distill_loss", loss, st, None, g)
         return loss, st, g
 
     def backward(self, stats, grad_out):
-        g = torch.empty(self.lead + (self.V,), dtype=self.logits.dtype, device=self.device)
+        g = _like(self.given)
         if self.rows:
             self._call("dnag_distill_backward", None, stats, grad_out.to(torch.float32).contiguous(), g)
         return g
@@ -504,7 +517,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[N
     index = _device(logits, u, *rows)
     lg, stride = _rows2d(logits)
     uc = u.contiguous()
-    out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    out = torch.empty_like(uc, dtype=torch.int64)
     n, V = lg.shape
     if n:
         t, k, p, q = numbers
