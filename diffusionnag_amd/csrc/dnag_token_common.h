@@ -107,8 +107,8 @@ static inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // launches there first (two threads racing set the same value twice)
 struct LdsLimit {
     std::atomic<size_t> have[64] = {};
-    int allow(const void *kern, size_t bytes) {
-        if (bytes <= 65536) return 0;
+    int allow(const void *kern, size_t bytes, size_t beside = 0) {     // `beside`: the kernel's static share
+        if (bytes + beside <= 65536) return 0;
         int dev = 0;
         TOK_TRY(hipGetDevice(&dev));
         if (dev < 64 && have[dev].load(std::memory_order_acquire) >= bytes) return 0;

@@ -551,6 +551,21 @@ def test_sample_few_rows_as_many(dtype):
         assert torch.equal(ops.sample_tokens(x[:9], u[:9], **some), ops.sample_tokens(x, u, **settings)[:9]), f"{settings}"
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_largest_vocab(dtype):
+    g = gen(20)
+    x = rnd(g, 2, 1 << 20, dtype=dtype, std=2.5)
+    x[1] = 0.0
+    x[1, -1] = 0.5
+    u = torch.tensor([0.3, 0.9999999])
+    for settings in (dict(), dict(top_k=100), dict(top_p=0.9), dict(temperature=0.0), dict(top_k=5000, top_p=0.7, min_p=0.01)):
+        full = {**dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **settings}
+        got = ops.sample_tokens(dev(x), dev(u), **settings)
+        assert got.cpu().tolist() == want_tokens(x, u, **full), f"{settings}"
+        many = ops.sample_tokens(dev(x).repeat(33, 1), dev(u).repeat(33), **settings)
+        assert torch.equal(many.view(33, 2), got.expand(33, 2)), f"{settings}"
+
+
 def test_sample_frequencies():
     """2^16 draws of one row: each token's count within six standard deviations of its probability."""
     x = torch.tensor([0.3, -1.0, 2.0, 1.9, 0.0, -3.0, 1.0])
@@ -743,6 +758,46 @@ def test_captured_and_replayed():
             graphs[k].replay()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(outs[k], want)), f"replay {seed} of graph {k}"
+
+
+def test_shared_rows_captured_and_on_two_streams():
+    """Drawing from few long rows keeps sums in a workspace: two captured graphs replayed in turn on changed logits, and two streams at
+    once, against one call at a time."""
+    settings = (dict(), dict(top_k=60, top_p=0.9), dict(top_p=0.8), dict(min_p=0.01, temperature=2.0))
+
+    def inputs(seed):
+        g = gen(seed)
+        return dev(rnd(g, 3, 70001, std=2.5)), dev(torch.rand(3, generator=g))
+
+    def draw(x, u):
+        return torch.stack([ops.sample_tokens(x, u, **s) for s in settings])
+    static = [inputs(1), inputs(2)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        draw(*static[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in static:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(draw(*s))
+        graphs.append(gr)
+    for seed in (3, 5, 7):
+        new = [inputs(seed), inputs(seed + 1)]
+        want = [draw(*n) for n in new]
+        for k in (0, 1):
+            for t, n in zip(static[k], new[k]):
+                t.copy_(n)
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), f"replay {seed}"
+        got = []
+        for n, stream in zip(new, (side, torch.cuda.Stream())):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append([draw(*n) for _ in range(4)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for many, w in zip(got, want) for o in many), f"streams {seed}"
 
 
 def test_captured_training_step_through_autograd():
