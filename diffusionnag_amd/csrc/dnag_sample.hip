@@ -983,5 +983,20 @@ extern "C" int dnag_sample_tokens(const dnag_sample_args *p) {
         a.ws_row = space_of_row(a.V);
     }
     hipStream_t st = (hipStream_t)p->stream;
-    return p->dtype == DNAG_F32 ? launch<float>(a, st) : p->dtype == DNAG_BF16 ? launch<tbf16>(a, st) : launch<tf16>(a, st);
+    constexpr int64_t MOST = 1 << 21;                  // rows of a launch: 2^32 lanes are more than a grid holds
+    const int64_t row_bytes = a.ld * (p->dtype == DNAG_F32 ? 4 : 2);
+    while (a.rows > 0) {
+        const int64_t left = a.rows - MOST;
+        if (left > 0) a.rows = MOST;
+        if (int rc = p->dtype == DNAG_F32 ? launch<float>(a, st) : p->dtype == DNAG_BF16 ? launch<tbf16>(a, st) : launch<tf16>(a, st)) return rc;
+        a.logits = (const char *)a.logits + MOST * row_bytes;
+        a.u += MOST;
+        a.out += MOST;
+        if (a.temperature) a.temperature += MOST;
+        if (a.top_k) a.top_k += MOST;
+        if (a.top_p) a.top_p += MOST;
+        if (a.min_p) a.min_p += MOST;
+        a.rows = left;
+    }
+    return 0;
 }

@@ -566,6 +566,18 @@ def test_sample_largest_vocab(dtype):
         assert torch.equal(many.view(33, 2), got.expand(33, 2)), f"{settings}"
 
 
+def test_sample_more_rows_than_a_launch():
+    n = (1 << 21) + 5
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(n, 65, generator=g, device=DEV).half()
+    u = torch.rand(n, generator=g, device=DEV)
+    rows = dict(temperature=torch.rand(n, generator=g, device=DEV) + 0.5, top_k=torch.randint(0, 9, (n,), generator=g, device=DEV, dtype=torch.int32),
+                top_p=torch.rand(n, generator=g, device=DEV) + 0.2, min_p=torch.rand(n, generator=g, device=DEV) * 0.2)
+    got = ops.sample_tokens(x, u, **rows)
+    for part in (slice(0, 1000), slice(n - 1000, n)):
+        assert torch.equal(got[part], ops.sample_tokens(x[part], u[part], **{k: v[part] for k, v in rows.items()}))
+
+
 def test_sample_frequencies():
     """2^16 draws of one row: each token's count within six standard deviations of its probability."""
     x = torch.tensor([0.3, -1.0, 2.0, 1.9, 0.0, -3.0, 1.0])
