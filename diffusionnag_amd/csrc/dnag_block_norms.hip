@@ -417,6 +417,7 @@ template <class TX, class TY, int TPR, int NV, bool LN>
 int launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
     // a team above 64 lanes is the workgroup: whole waves, as many as the row needs (4100 columns: 9, not 16)
     const int threads = TPR <= 64 ? 256 : NV > 1 ? TPR : (int)(ceil_div(a.d, 512) * 64);
+    if (int rc = grid_fits(blocks, threads)) return rc;
     if (grad) {
         const size_t lds = NV == 1 ? (size_t)3 * threads * 32 : 0;
         static LdsLimit limit;

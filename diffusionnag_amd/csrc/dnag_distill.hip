@@ -286,6 +286,7 @@ int launch(const DistillArgs &a, hipStream_t st) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1;
     const int64_t lanes = NV > 0 ? ceil_div(a.V, 8 * NV) : TPR;        // a team above 64 lanes: whole waves, as many as the row fills
     const unsigned threads = TPR <= 64 ? 256 : (unsigned)(ceil_div(lanes, 64) * 64);
+    if (int rc = grid_fits(ceil_div(a.rows, NT), threads)) return rc;
     hipLaunchKernelGGL((distill_kernel<T, TPR, NV, MODE>), dim3((unsigned)ceil_div(a.rows, NT)), dim3(threads), (size_t)NT * a.K * 12, st, a);
     TOK_TRY(hipGetLastError());
     return 0;

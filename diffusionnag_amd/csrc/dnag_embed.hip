@@ -382,6 +382,7 @@ template <class T, class I>
 int forward_t(const void *ids, int64_t rows, const void *w, int64_t ws, int64_t V, int64_t d, float scale, void *out, hipStream_t st) {
     const int tpr = pow2_at_least(ceil_div(d, 8), 1, 256);
     const int64_t bx = ceil_div(rows, 256 / tpr);
+    if (int rc = grid_fits(bx, 256)) return rc;
     hipLaunchKernelGGL((embed_forward_kernel<T, I>), dim3((unsigned)bx, (unsigned)ceil_div(d, (int64_t)tpr * 8)), dim3(256), 0, st,
                        (const I *)ids, rows, (const T *)w, ws, V, (int)d, scale, (T *)out, tpr);
     TOK_TRY(hipGetLastError());
@@ -449,7 +450,7 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
     // (a chunk's number fits: at least 8 rows each)
     const int jtile = (int)ceil_div(d, 256);
     const int64_t joins = p.nchunk * (int64_t)jtile;
-    if (joins > 0x7ff00000ll) return dnag_fail(DNAG_E_ARG, "rows=%lld x dim=%lld: too many pieces for one launch", (long long)rows, (long long)d);
+    if (int rc = grid_fits(joins + 1024, 512)) return rc;
     const int64_t clear = p.passes > 1 ? 0 : V < 1024 ? V : 1024;
     const EmbFill f = {last, (uint16_t *)out, 0, V, d * (int64_t)(sizeof(T) / 2), (int)joins};
     hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)(joins + clear)), dim3(512), 0, st, key[now], last, rows, (uint32_t)V, part, p.chunk, jtile, (int)d, scale,

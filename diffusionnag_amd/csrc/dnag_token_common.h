@@ -103,6 +103,11 @@ static inline bool dtype_known(int t) { return t == DNAG_F32 || t == DNAG_BF16 |
 static inline size_t dtype_bytes(int t) { return t == DNAG_F32 ? 4 : 2; }
 static inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// a grid holds less than 2^32 lanes along x
+static inline int grid_fits(int64_t blocks, int64_t threads) {
+    return blocks * threads < (1ll << 32) ? 0 : dnag_fail(DNAG_E_ARG, "%lld workgroups of %lld lanes: too many rows for one launch", (long long)blocks, (long long)threads);
+}
+
 // the largest dynamic LDS a kernel may ask for is a per-device setting: set once per (kernel, device), from whichever thread
 // launches there first (two threads racing set the same value twice)
 struct LdsLimit {

@@ -143,6 +143,7 @@ def test_c_entries_check_before_they_launch():
     refused(e(P, 8, 1, P, 8, 0, 8, 0, 1.0, P, None), "num_tokens")
     refused(e(P, 8, 1, P, 8, 4, 0, 0, 1.0, P, None), "dim")
     refused(e(None, 8, 1, P, 8, 4, 8, 0, 1.0, P, None), "NULL")
+    refused(e(P, 8, 0x7fffffff, P, 4096, 4, 4096, 0, 1.0, P, None), "too many rows")
     assert e(None, 8, 0, None, 8, 4, 8, 0, 1.0, None, None) == 0                      # no rows: nothing to do
     need = lib.dnag_embed_grad_workspace_bytes(1000, 500, 64)
     assert need > 0
@@ -187,6 +188,9 @@ def test_c_entries_check_before_they_launch():
     refused(lib.dnag_distill_loss_grad(C.byref(distill(grad=None))), "NULL")
     refused(lib.dnag_distill_backward(C.byref(distill(stats=None))), "NULL")
     refused(lib.dnag_distill_backward(C.byref(distill(grad_out=None))), "NULL")
+
+    refused(lib.dnag_distill_loss(C.byref(distill(rows=0x7fffffff, vocab=1000, logits_stride=1000, reduction=0, workspace_bytes=1 << 40))), "too many rows")
+    refused(lib.dnag_block_norms_forward(C.byref(norms(rows=0x7fffffff, gate_rows=1, dim=4096, x_stride=4096, y_stride=4096))), "too many rows")
 
     def sample(**kw):
         a = _lib.SampleArgsC()
