@@ -11,7 +11,8 @@ contiguous last dimension are read in place, others are copied first; outputs ar
 allocator and belong to the call (also under graph capture).  The first three are differentiable through ``torch.autograd``;
 ``embed_tokens_grad``, ``block_norms_grad`` and ``distill_loss_and_grad`` give the same gradients without it, which is also how to
 capture a training step into a graph: a backward pass of ``torch.autograd`` that is captured while an eager graph of the
-same leaves is alive ends the process inside torch, so the differentiable calls raise there.
+same leaves is alive ends the process inside torch, so the differentiable calls raise there.  There is no forward-mode
+derivative: arguments that carry a tangent are refused.
 Element types: float32, bfloat16, float16.  All sums and statistics are float32 or wider; results are rounded once.
 """
 
@@ -20,6 +21,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -98,6 +100,17 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors of forward-mode differentiation: the operators have no tangents, and a result without one would count as
+    a derivative of zero.  (Outside a dual level there are none: 0.1 us.)"""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the token operators have no forward-mode derivative: an argument carries a tangent (differentiate backward, or "
+                               "take the primal out with torch.autograd.forward_ad.unpack_dual)")
+
+
 def _leaf_mark(*tensors: Optional[torch.Tensor]) -> None:
     """Refuses to record a backward pass of leaves under graph capture while an eager graph of the same leaves is alive: their
     gradient accumulators belong to the eager graph's stream, and running them inside the capture ends the process."""
@@ -157,6 +170,7 @@ def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: Number = 1.0
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [num_tokens, dim], got {tuple(weight.shape)}")
     _dtype(weight, "weight")
+    _no_tangents(weight)
     ids = _check_ids(ids)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {weight.shape[0] - 1}")
@@ -178,6 +192,7 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
     if num_tokens < 1 or grad.shape[-1] < 1:
         raise ValueError(f"num_tokens={num_tokens}, dim={grad.shape[-1]}: both must be positive")
     code = _dtype(grad, "grad")
+    _no_tangents(grad)
     index = _device(grad, ids)
     g, stride = _rows2d(grad)
     rows, d = g.shape
@@ -361,6 +376,7 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, ...): every G-th part of the rows of ``x``, in order,
     uses one.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    _no_tangents(*tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _leaf_mark(*tensors)
         out = _BlockNorms.apply(*tensors, residual_scale, norm, eps, pre, dtype)
@@ -378,6 +394,7 @@ def block_norms_grad(grad_x: Optional[torch.Tensor], grad_h: Optional[torch.Tens
                      dtype: Optional[torch.dtype] = None) -> BlockNormsGrad:
     """Gradients of ``block_norms`` (same arguments) for ``grad_x`` and ``grad_h``, the gradients of ``x_new`` and ``h`` (None: zero).
     Nothing of the forward pass but its inputs is needed.  Sums over rows run in one fixed order."""
+    _no_tangents(grad_x, grad_h, x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     seam = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype)
     return seam.backward(grad_x, grad_h, _SMALL)
 
@@ -468,6 +485,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     teacher or the weights: they must not require one."""
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
         raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")
+    _no_tangents(logits, teacher_logits, row_weight)
     if logits.requires_grad and torch.is_grad_enabled():
         _leaf_mark(logits)
         return _DistillLoss.apply(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction)
@@ -478,6 +496,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
                           row_weight: Optional[torch.Tensor] = None, reduction: str = "mean"):
     """``distill_loss`` and its gradient with respect to ``logits`` (for an upstream gradient of 1) in one pass over the logits: two
     thirds of the memory traffic of the loss followed by its backward pass.  Returns ``(loss, grad)``."""
+    _no_tangents(logits, teacher_logits, row_weight)
     loss, _, grad = _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss(grad=True)
     return loss, grad
 

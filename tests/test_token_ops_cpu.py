@@ -223,3 +223,35 @@ def test_eager_graph_of_the_same_leaf_is_noticed(monkeypatch):
         ops._leaf_mark(w)
     del alive
     ops._leaf_mark(w)
+
+
+# calls of every differentiable operator and explicit gradient with one argument given, the others plain
+IDS, TIDS = torch.tensor([0, 2, 1]), torch.tensor([[0, 1], [2, -1], [3, 3]])
+DIFFERENTIABLE = {
+    "embedding weight": ((4, 8), lambda t: ops.embed_tokens(IDS, t)),
+    "embedding grad": ((3, 8), lambda t: ops.embed_tokens_grad(t, IDS, 4)),
+    "norms x": ((3, 8), lambda t: ops.block_norms(t, torch.ones(3, 8))),
+    "norms x alone": ((3, 8), lambda t: ops.block_norms(t)),
+    "norms y": ((3, 8), lambda t: ops.block_norms(torch.ones(3, 8), t)),
+    "norms gate": ((8,), lambda t: ops.block_norms(torch.ones(3, 8), torch.ones(3, 8), gate=t)),
+    "norms weight": ((8,), lambda t: ops.block_norms(torch.ones(3, 8), torch.ones(3, 8), post_weight=t)),
+    "norms bias": ((8,), lambda t: ops.block_norms(torch.ones(3, 8), torch.ones(3, 8), norm="layer", pre_bias=t)),
+    "norms grad": ((3, 8), lambda t: ops.block_norms_grad(None, t, torch.ones(3, 8))),
+    "norms grad's x": ((3, 8), lambda t: ops.block_norms_grad(None, torch.ones(3, 8), t)),
+    "distillation": ((3, 8), lambda t: ops.distill_loss(t, TIDS, torch.ones(3, 2))),
+    "distillation teacher": ((3, 2), lambda t: ops.distill_loss(torch.ones(3, 8), TIDS, t)),
+    "distillation weight": ((3,), lambda t: ops.distill_loss(torch.ones(3, 8), TIDS, torch.ones(3, 2), row_weight=t)),
+    "distillation step": ((3, 8), lambda t: ops.distill_loss_and_grad(t, TIDS, torch.ones(3, 2))),
+}
+
+
+@pytest.mark.parametrize("what", DIFFERENTIABLE)
+def test_tangents_are_refused(what):
+    """A dual tensor has requires_grad False: taken for a plain one, the result would have no tangent, a derivative of zero."""
+    from torch.autograd import forward_ad
+    shape, call = DIFFERENTIABLE[what]
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(forward_ad.make_dual(torch.ones(shape), torch.ones(shape)))
+        with pytest.raises(RuntimeError, match="no CPU fallback"):          # a plain tensor inside the level comes as far as ever
+            call(torch.ones(shape))
