@@ -12,7 +12,8 @@ allocator and belong to the call (also under graph capture).  The first three ar
 ``embed_tokens_grad``, ``block_norms_grad`` and ``distill_loss_and_grad`` give the same gradients without it, which is also how to
 capture a training step into a graph: a backward pass of ``torch.autograd`` that is captured while an eager graph of the
 same leaves is alive ends the process inside torch, so the differentiable calls raise there.  There is no forward-mode
-derivative: arguments that carry a tangent are refused.
+derivative: arguments that carry a tangent are refused.  So are torch.jit.trace and make_fx, which would record an empty result;
+torch.compile breaks its graph around the calls.
 Element types: float32, bfloat16, float16.  All sums and statistics are float32 or wider; results are rounded once.
 """
 
@@ -21,6 +22,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Union
 
 import torch
+from torch._ops import mode_stack_state_for_pre_dispatch
 from torch.autograd import forward_ad
 
 from . import _lib
@@ -30,6 +32,8 @@ _REDUCE = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE
 _IDS = {torch.int32: 4, torch.int64: 8}
 
 _MOST = 1.7976931348623157e308
+
+_pre_dispatch_modes = mode_stack_state_for_pre_dispatch()
 
 Number = Union[int, float]
 
@@ -100,6 +104,14 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _not_recorded() -> None:
+    """Refuses to be recorded by torch.jit.trace and make_fx: they would see the allocation of the result and not the launch that fills
+    it, and the recorded program would return memory as it is.  (Three reads of thread-local state, 0.4 us.)"""
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None) \
+            or _pre_dispatch_modes.get(0) is not None:         # 0: the recording mode's place
+        raise RuntimeError("the token operators cannot be recorded by torch.jit.trace or make_fx: call them, or capture the calls into a HIP graph")
+
+
 def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
     """Refuses dual tensors of forward-mode differentiation: the operators have no tangents, and a result without one would count as
     a derivative of zero.  (Outside a dual level there are none: 0.1 us.)"""
@@ -167,6 +179,7 @@ def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: Number = 1.0
 
     ``ids`` outside ``0 .. len(weight) - 1`` (the -1 or -100 of a padded batch, another shard's tokens) give rows of zeros and
     take no part in the gradient; ``padding_idx`` is looked up but takes no part in the gradient (as in torch)."""
+    _not_recorded()
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [num_tokens, dim], got {tuple(weight.shape)}")
     _dtype(weight, "weight")
@@ -185,6 +198,7 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
                       padding_idx: Optional[int] = None) -> torch.Tensor:
     """Gradient of ``embed_tokens`` with respect to ``weight`` ([num_tokens, d], the type of ``grad``): the rows of ``grad``
     summed by token in float32, in the order of the tokens' positions, the same bits every time."""
+    _not_recorded()
     lib = _lib.load()
     ids = _check_ids(ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
@@ -376,6 +390,7 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, ...): every G-th part of the rows of ``x``, in order,
     uses one.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    _not_recorded()
     _no_tangents(*tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _leaf_mark(*tensors)
@@ -394,6 +409,7 @@ def block_norms_grad(grad_x: Optional[torch.Tensor], grad_h: Optional[torch.Tens
                      dtype: Optional[torch.dtype] = None) -> BlockNormsGrad:
     """Gradients of ``block_norms`` (same arguments) for ``grad_x`` and ``grad_h``, the gradients of ``x_new`` and ``h`` (None: zero).
     Nothing of the forward pass but its inputs is needed.  Sums over rows run in one fixed order."""
+    _not_recorded()
     _no_tangents(grad_x, grad_h, x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     seam = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype)
     return seam.backward(grad_x, grad_h, _SMALL)
@@ -483,6 +499,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     or their type's lowest value have no probability (a row of nothing but lowest values: one and the same probability).
     ``temperature`` is 1e-6 to 1e6 (float16 logits: from 0.1 on).  No gradient reaches the
     teacher or the weights: they must not require one."""
+    _not_recorded()
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
         raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")
     _no_tangents(logits, teacher_logits, row_weight)
@@ -496,6 +513,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
                           row_weight: Optional[torch.Tensor] = None, reduction: str = "mean"):
     """``distill_loss`` and its gradient with respect to ``logits`` (for an upstream gradient of 1) in one pass over the logits: two
     thirds of the memory traffic of the loss followed by its backward pass.  Returns ``(loss, grad)``."""
+    _not_recorded()
     _no_tangents(logits, teacher_logits, row_weight)
     loss, _, grad = _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss(grad=True)
     return loss, grad
@@ -514,6 +532,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[N
     index.  The token is the first one, in index order, whose running sum of kept probability exceeds ``u`` times the total.
     NaN and -inf are never drawn; a row of nothing else gives -1.  Each setting is a number, or a tensor with a value per
     row (float32; int32 for ``top_k``).  The same inputs give the same tokens, whatever else runs.  vocab <= 2^20."""
+    _not_recorded()
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
     lead = logits.shape[:-1]

@@ -255,3 +255,27 @@ def test_tangents_are_refused(what):
             call(forward_ad.make_dual(torch.ones(shape), torch.ones(shape)))
         with pytest.raises(RuntimeError, match="no CPU fallback"):          # a plain tensor inside the level comes as far as ever
             call(torch.ones(shape))
+
+
+RECORDED = {**DIFFERENTIABLE, "drawing": ((3, 8), lambda t: ops.sample_tokens(t, torch.zeros(3)))}
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("recorder", ["jit", "fx", "fx before dispatch", "fx fake"])
+@pytest.mark.parametrize("what", RECORDED)
+def test_recording_is_refused(what, recorder, grad, monkeypatch):
+    """torch.jit.trace and make_fx see the allocation of the result and not the launch (stubbed here) that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    shape, call = RECORDED[what]
+    grad = grad and what not in ("distillation teacher", "distillation weight")         # those must not require one
+    monkeypatch.setattr(ops, "_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_launch", lambda *a: None)
+    monkeypatch.setattr(ops, "_leaf_mark", lambda *t: None)
+    t = torch.ones(shape, requires_grad=grad)
+    call(t)                                                                 # not recorded: as ever
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        if recorder == "jit":
+            torch.jit.trace(call, t, check_trace=False)
+        else:
+            make_fx(call, tracing_mode="fake" if recorder == "fx fake" else "real", pre_dispatch=recorder == "fx before dispatch")(t)
+    call(t)
