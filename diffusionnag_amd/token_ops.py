@@ -243,6 +243,21 @@ def _small(t: Optional[torch.Tensor], name: str, d: int, dtype) -> Optional[torc
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _check_gate(gate: torch.Tensor, x: torch.Tensor) -> None:
+    """The kernels give each row of the gate a run of consecutive rows of ``x``.  Refuses shapes that say something else: a dimension that
+    the gate repeats over, in front of one that it does not ([1, N, d] beside [B, N, d], [N, d] beside [B, N, d])."""
+    lead, own = x.shape[:-1], gate.shape[:-1]
+    over = len(lead) - len(own)
+    if over >= 0 and all(g == 1 or g == n for g, n in zip(own, lead[over:])):                # broadcasts
+        repeats = [g == 1 and n != 1 for g, n in zip((1,) * over + tuple(own), lead)]
+        own = (1,) * over + tuple(own)
+    else:                                                                                   # a list of rows
+        repeats = [g == 1 for g in own]
+    if any(r and any(g != 1 for g in own[k:]) for k, r in enumerate(repeats)):
+        raise ValueError(f"gate {tuple(gate.shape)} beside x {tuple(x.shape)} repeats over a dimension in front of its own rows; built is a row for each run of "
+                         "consecutive rows ([B, 1, d], [d]) or for each row (expand the gate to the shape of x)")
+
+
 class _Seam:
     """The checked arguments of one ``block_norms`` call as the library takes them."""
     __slots__ = ("index", "shape", "device", "dtype", "given_x", "given_y", "x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "rows", "d", "pre", "head",
@@ -296,6 +311,8 @@ class _Seam:
         if gate is not None:
             if gate.shape[-1:] != (d,) or (gate.dtype != dtype and gate.dtype != f32):
                 raise ValueError(f"gate must be [..., {d}] of type {dtype} or float32, got {tuple(gate.shape)} {gate.dtype}")
+            if gate.dim() > 1 and not gate.dim() == x.dim() == 2:
+                _check_gate(gate, x)
             gate_rows = gate.numel() // d
             if gate_rows < 1 or rows % gate_rows:
                 raise ValueError(f"{rows} rows do not divide into {gate_rows} gate rows")
@@ -387,8 +404,9 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     ``x`` [..., d] is the residual stream (the branch's type, or float32 beside a 16-bit branch), ``y`` the block's output.
     ``norm``: 'rms' (no bias) or 'layer'.  ``y=None`` is the entry of the first block: ``(x, N_pre(x))``, with ``dtype`` the type of
     ``h`` (default: that of ``x``); ``pre=False`` the exit of the last one: ``(x_new, None)``.  ``h`` is computed from
-    the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, ...): every G-th part of the rows of ``x``, in order,
-    uses one.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
+    the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, a list [G, d], ...): every
+    G-th part of the rows of ``x``, in order, uses one.  A gate that broadcasting would repeat over a leading dimension ([1, N, d] or [N, d] beside
+    [B, N, d]) is refused: expand it to the shape of ``x``.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     _not_recorded()
     _no_tangents(*tensors)

@@ -279,3 +279,29 @@ def test_recording_is_refused(what, recorder, grad, monkeypatch):
         else:
             make_fx(call, tracing_mode="fake" if recorder == "fx fake" else "real", pre_dispatch=recorder == "fx before dispatch")(t)
     call(t)
+
+
+@pytest.mark.parametrize("gate,x,fits", [
+    ((8,), (6, 4, 8), True), ((1, 8), (6, 4, 8), True), ((1, 1, 8), (6, 4, 8), True), ((6, 1, 8), (6, 4, 8), True), ((6, 4, 8), (6, 4, 8), True),
+    ((2, 3, 1, 8), (2, 3, 4, 8), True), ((2, 1, 1, 8), (2, 3, 4, 8), True), ((4, 8), (1, 4, 8), True), ((1, 4, 8), (1, 4, 8), True),
+    ((6, 8), (6, 4, 8), True), ((12, 8), (6, 4, 8), True), ((24, 8), (6, 4, 8), True), ((6, 8), (24, 8), True), ((1, 8), (8,), True),   # lists of rows
+    ((6, 1, 8), (24, 8), True), ((24, 1, 8), (6, 4, 8), True), ((6, 2, 8), (6, 4, 8), True),
+    ((1, 4, 8), (6, 4, 8), False), ((4, 8), (6, 4, 8), False), ((4, 8), (4, 4, 8), False),                    # a row for each position
+    ((2, 1, 4, 8), (2, 3, 4, 8), False), ((3, 1, 8), (2, 3, 4, 8), False), ((1, 3, 1, 8), (2, 3, 4, 8), False),
+    ((1, 4, 8), (24, 8), False), ((2, 1, 4, 8), (24, 8), False),                                             # neither broadcasts nor is a list
+])
+def test_gates_mean_runs_of_rows(gate, x, fits, monkeypatch):
+    """A gate that is taken means what torch's broadcasting makes of it, or is a list of rows: anything else is refused."""
+    monkeypatch.setattr(ops, "_leaf_mark", lambda *t: None)
+    a, g = torch.ones(x), torch.randn(gate, generator=torch.Generator().manual_seed(1))
+    for call in (lambda: ops.block_norms(a, a, gate=g), lambda: ops.block_norms(a, a, gate=g.clone().requires_grad_(True)), lambda: ops.block_norms_grad(a, a, a, a, gate=g)):
+        with pytest.raises(RuntimeError if fits else ValueError, match="no CPU fallback" if fits else "gate"):
+            call()
+    try:
+        broadcast = torch.broadcast_shapes(gate, x) == x
+    except RuntimeError:
+        broadcast = False
+    if fits and broadcast:                                             # the rows that the kernels use
+        rows = a.numel() // 8
+        used = g.reshape(-1, 8).repeat_interleave(rows // (g.numel() // 8), 0).reshape(x)
+        assert torch.equal(used, g.expand(x))
