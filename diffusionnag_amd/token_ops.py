@@ -314,7 +314,7 @@ class _Seam:
             if gate.dim() > 1 and not gate.dim() == x.dim() == 2:
                 _check_gate(gate, x)
             gate_rows = gate.numel() // d
-            if gate_rows < 1 or rows % gate_rows:
+            if rows and (gate_rows < 1 or rows % gate_rows):
                 raise ValueError(f"{rows} rows do not divide into {gate_rows} gate rows")
             if gate.dtype == f32:
                 small |= 1

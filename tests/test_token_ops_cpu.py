@@ -305,3 +305,15 @@ def test_gates_mean_runs_of_rows(gate, x, fits, monkeypatch):
         rows = a.numel() // 8
         used = g.reshape(-1, 8).repeat_interleave(rows // (g.numel() // 8), 0).reshape(x)
         assert torch.equal(used, g.expand(x))
+
+
+@pytest.mark.parametrize("x,gate", [((0, 4, 8), (0, 1, 8)), ((0, 4, 8), (0, 4, 8)), ((0, 8), (0, 8)), ((0, 4, 8), (8,)), ((0, 4, 8), (3, 1, 8)), ((5, 0, 8), (5, 1, 8))])
+def test_empty_batches_with_a_gate(x, gate, monkeypatch):
+    """No rows: empty results and gradients of zeros, nothing is launched, whatever number of gate rows goes with them."""
+    monkeypatch.setattr(ops, "_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_launch", None)
+    a, g = torch.ones(x), torch.ones(gate)
+    x_new, h = ops.block_norms(a, a, gate=g, pre_weight=torch.ones(8))
+    assert x_new.shape == h.shape == x
+    got = ops.block_norms_grad(a, a, a, a, gate=g, pre_weight=torch.ones(8))
+    assert got.x.shape == got.y.shape == x and got.gate.shape == gate and not got.gate.any() and got.pre_weight.shape == (8,) and not got.pre_weight.any()
