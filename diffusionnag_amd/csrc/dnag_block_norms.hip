@@ -421,7 +421,7 @@ int launch(const BnArgs &a, bool grad, unsigned blocks, hipStream_t st) {
     if (grad) {
         const size_t lds = NV == 1 ? (size_t)3 * threads * 32 : 0;
         static LdsLimit limit;
-        if (int rc = limit.allow((const void *)block_norms_grad_kernel<TX, TY, TPR, NV, LN>, lds)) return rc;
+        TOK_TRY(limit.allow((const void *)block_norms_grad_kernel<TX, TY, TPR, NV, LN>, lds));
         hipLaunchKernelGGL((block_norms_grad_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(threads), lds, st, a);
     } else hipLaunchKernelGGL((block_norms_kernel<TX, TY, TPR, NV, LN>), dim3(blocks), dim3(threads), 0, st, a);
     return 0;

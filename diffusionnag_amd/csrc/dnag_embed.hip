@@ -398,7 +398,7 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
         const size_t lds = (size_t)32 * V * 64 * 4;
         auto kern = embed_few_kernel<T, I>;
         static LdsLimit limit;
-        if (int rc = limit.allow((const void *)kern, lds)) return rc;
+        TOK_TRY(limit.allow((const void *)kern, lds));
         float *part = p.nblk > 1 ? (float *)ws : nullptr;
         hipLaunchKernelGGL(kern, dim3(p.nblk, (unsigned)ceil_div(d, 64)), dim3(256), lds, st, id, rows, g, gs, (int)V, pad, (int)d, scale, p.per_block, part, (T *)out);
         TOK_TRY(hipGetLastError());
@@ -417,7 +417,7 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
         while (n2 < rows) n2 *= 2;
         auto kern = embed_sort_lds_kernel<I>;
         static LdsLimit limit;
-        if (int rc = limit.allow((const void *)kern, (size_t)n2 * 8)) return rc;
+        TOK_TRY(limit.allow((const void *)kern, (size_t)n2 * 8));
         const unsigned zero = (unsigned)(ceil_div(V, 4096) < 256 ? ceil_div(V, 4096) : 256);
         hipLaunchKernelGGL(kern, dim3(1 + zero), dim3(1024), (size_t)n2 * 8, st, id, (int)rows, n2, V, pad, key[0], pos[0], last);
         TOK_TRY(hipGetLastError());

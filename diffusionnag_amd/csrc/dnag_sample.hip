@@ -937,7 +937,7 @@ template <class T, bool SPLIT>
 int launch_long(const SampleArgs &a, hipStream_t st) {
     const size_t bytes = (size_t)ws_pieces(a.V) * 8 + (__is_same(T, tbf16) ? 5120 * 8 : 0);      // pieces, and the slots' weights
     static LdsLimit limit;
-    if (int rc = limit.allow((const void *)sample_row_kernel<T, 1024, SPLIT>, bytes, 52 * 1024)) return rc;
+    TOK_TRY(limit.allow((const void *)sample_row_kernel<T, 1024, SPLIT>, bytes, 52 * 1024));
     hipLaunchKernelGGL((sample_row_kernel<T, 1024, SPLIT>), dim3((unsigned)a.rows), dim3(1024), bytes, st, a);
     return 0;
 }

@@ -4,8 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stddef.h>
-#include <atomic>
 #include "../../include/dnag.h"
+#include "dnag_lds_limit.h"
 
 // defined in dnag_lib.hip: formats dnag_last_error() of the calling thread and returns `code`
 __attribute__((visibility("hidden"))) int dnag_fail(int code, const char *fmt, ...);
@@ -107,21 +107,6 @@ static inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 static inline int grid_fits(int64_t blocks, int64_t threads) {
     return blocks * threads < (1ll << 32) ? 0 : dnag_fail(DNAG_E_ARG, "%lld workgroups of %lld lanes: too many rows for one launch", (long long)blocks, (long long)threads);
 }
-
-// the largest dynamic LDS a kernel may ask for is a per-device setting: set once per (kernel, device), from whichever thread
-// launches there first (two threads racing set the same value twice)
-struct LdsLimit {
-    std::atomic<size_t> have[64] = {};
-    int allow(const void *kern, size_t bytes, size_t beside = 0) {     // `beside`: the kernel's static share
-        if (bytes + beside <= 65536) return 0;
-        int dev = 0;
-        TOK_TRY(hipGetDevice(&dev));
-        if (dev < 64 && have[dev].load(std::memory_order_acquire) >= bytes) return 0;
-        TOK_TRY(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        if (dev < 64) have[dev].store(bytes, std::memory_order_release);
-        return 0;
-    }
-};
 
 // orders LDS accesses of a wave's lanes against each other (they run in step; this keeps the compiler from moving them)
 __device__ __forceinline__ void wave_fence() {

@@ -2,6 +2,8 @@
 check before they touch the device)."""
 
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -317,3 +319,51 @@ def test_empty_batches_with_a_gate(x, gate, monkeypatch):
     assert x_new.shape == h.shape == x
     got = ops.block_norms_grad(a, a, a, a, gate=g, pre_weight=torch.ones(8))
     assert got.x.shape == got.y.shape == x and got.gate.shape == gate and not got.gate.any() and got.pre_weight.shape == (8,) and not got.pre_weight.any()
+
+
+LDS_RACE = r"""
+#include "dnag_lds_limit.h"
+#include <chrono>
+#include <stdio.h>
+#include <thread>
+// The driver's side: one kernel, one device.  The call with the smaller value takes effect after the one with the larger, if the two overlap.
+static std::atomic<size_t> limit{65536};
+static std::atomic<int> inside{0}, smaller_done{0}, calls{0};
+extern "C" hipError_t hipGetDevice(int *d) { *d = 0; return hipSuccess; }
+extern "C" hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int bytes) {
+    ++calls;
+    ++inside;
+    for (int i = 0; i < 100 && inside < 2; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(2));     // time for the other one to come
+    if (bytes == 80 * 1024) {
+        std::this_thread::sleep_for(std::chrono::milliseconds(50));
+        limit = bytes;
+        smaller_done = 1;
+        return hipSuccess;
+    }
+    limit = bytes;
+    for (int i = 0; i < 100 && inside == 2 && !smaller_done; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(2));
+    return hipSuccess;
+}
+int main() {
+    static LdsLimit a;
+    std::thread small([] { a.allow(nullptr, 80 * 1024); }), large([] { a.allow(nullptr, 120 * 1024); });
+    small.join();
+    large.join();
+    const int before = calls;
+    a.allow(nullptr, 120 * 1024);                      // recorded: nothing to set
+    a.allow(nullptr, 60 * 1024);
+    a.allow(nullptr, 60 * 1024, 8 * 1024);
+    printf("%zu %d\n", limit.load(), calls.load() - before);
+}
+"""
+
+
+def test_two_first_calls_leave_the_larger_lds_limit(tmp_path):
+    """Two threads that ask for different amounts of LDS at once: the larger one has to be set in the end, since it is what is recorded."""
+    src, exe = tmp_path / "race.cpp", tmp_path / "race"
+    src.write_text(LDS_RACE)
+    csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{csrc}", str(src), "-o", str(exe)], check=True)
+    for _ in range(3):
+        out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.split()
+        assert out == [str(120 * 1024), "0"], out
