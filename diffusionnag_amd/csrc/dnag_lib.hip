@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "dnag_common.h"
+#include "dnag_lds_limit.h"
 #include "dnag_encoder.hip.h"
 #include "dnag_encoder8.hip.h"
 #include "dnag_head.hip.h"
@@ -568,19 +569,9 @@ extern "C" int dnag_timing_end(void) {
     return 0;
 }
 
-// hipFuncAttributeMaxDynamicSharedMemorySize is a per-device setting: set it once per (kernel, device), from whichever
-// thread launches first there (two threads racing set the same value twice)
-struct LdsAttr {
-    std::atomic<size_t> bytes[64];
-    LdsAttr() { for (auto &b : bytes) b.store(0); }
-};
-static int ensure_lds(LdsAttr &a, const void *kern, size_t bytes) {
-    int dev = 0;
-    HIP_TRY(hipGetDevice(&dev));
-    std::atomic<size_t> &have = a.bytes[dev & 63];
-    if (have.load(std::memory_order_acquire) >= bytes) return 0;
-    HIP_TRY(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    have.store(bytes, std::memory_order_release);
+// always set, whatever the kernel's static share is
+static int ensure_lds(LdsLimit &a, const void *kern, size_t bytes) {
+    HIP_TRY(a.allow(kern, bytes, 65536));
     return 0;
 }
 
@@ -629,7 +620,7 @@ static int launch_gemm(const float *A, const float *W, const float *bias, float 
     auto k7 = gemm_dma_kernel<ACT_ELU, false, 7, true>;      // final.linears.1 + final.linears.2 fused, NAS-Bench-201
     auto k9 = gemm_dma_kernel<ACT_ELU, false, 9, true>;      // same, OFA
     auto k0 = gemm_dma_kernel<ACT_ELU, true, 0, true>;
-    static LdsAttr a7, a9, a0;
+    static LdsLimit a7, a9, a0;
     if (int rc = ensure_lds(a7, reinterpret_cast<const void *>(k7), Ge::lds_bytes)) return rc;
     if (int rc = ensure_lds(a9, reinterpret_cast<const void *>(k9), Ge::lds_bytes)) return rc;
     if (int rc = ensure_lds(a0, reinterpret_cast<const void *>(k0), Ge::lds_bytes)) return rc;
@@ -655,7 +646,7 @@ static int launch_gemm32(const float *A, int lda, const float *amax_a, const flo
         return fail(DNAG_E_ARG, "split gemm shape %zu x %d x %d (lda %d ldw %d split %d) not tile aligned", M, Nout, K, lda, ldw, splitk);
     if (splitk > 1 && (ACT != ACT_NONE || bias)) return fail(DNAG_E_ARG, "split-K gemm takes no bias / activation");
     auto kern = gemm_split_kernel<ACT, false, TAG, 0, true>;
-    static LdsAttr attr;
+    static LdsLimit attr;
     if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), Ge::lds_bytes)) return rc;
     SplitF32Args fa;
     fa.sc = nullptr;
@@ -681,7 +672,7 @@ static int launch_encoder_t(const CateLayout &lay, const float *P, const float *
     typedef EncGeom<N, G, 128> Ge;
     const size_t lds = Ge::lds_floats * sizeof(float);
     auto kern = encoder_kernel<N, V, G, 8, 128, true, false, false, true, true>;   // split-arithmetic linears, concat in split-pair rows
-    static LdsAttr attr;
+    static LdsLimit attr;
     if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
     const int grid = (batch + G - 1) / G;
     EncSave none;
@@ -700,7 +691,7 @@ static int launch_encoder8(const CateLayout &lay, const float *P, const float *x
     if (lay.d != Ge::D || lay.dff != Ge::DFF) return fail(DNAG_E_ARG, "encoder8: d_model %d / d_ff %d", lay.d, lay.dff);
     const size_t lds = Ge::lds_floats * sizeof(float);
     auto kern = encoder8_kernel<N, V>;
-    static LdsAttr attr;
+    static LdsLimit attr;
     if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
     EncSave nosave;
     DropMasks nodrop;
@@ -745,7 +736,7 @@ static int launch_predictor(const PredLayout &lay, const float *P, const float *
     typedef PredGeom<8, 7> Ge;
     const size_t lds = Ge::lds_bytes(lay.hs, lay.L);
     auto kern = predictor_kernel<8, 7>;
-    static LdsAttr attr;
+    static LdsLimit attr;
     if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
     const int grid = (batch + Ge::G - 1) / Ge::G;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(PRED_NW * 64), lds, st, P, lay, x, temb, tstride, mask, mstride, c0, y, grad, batch);
@@ -899,7 +890,7 @@ static int run_predcate(const PredCateLayout &y, const float *P, const float *x,
         typedef EncGeom<PC_N, PC_G, 32> Ge;
         const size_t lds = Ge::lds_floats * sizeof(float);
         auto kern = encoder_kernel<PC_N, PC_V, PC_G, 2, 32, false, true, false, false, true>;   // saved activations, split-arithmetic linears
-        static LdsAttr attr;
+        static LdsLimit attr;
         if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
         DropMasks nodrop;
         memset(&nodrop, 0, sizeof(nodrop));
@@ -957,7 +948,7 @@ static int run_predcate(const PredCateLayout &y, const float *P, const float *x,
         typedef PcbGeom<PC_N, PC_G, 2, 32> Ge;
         const size_t lds = Ge::lds_floats * sizeof(float);
         auto kern = predcate_enc_bwd_kernel<PC_N, PC_V, PC_G, 2, 32>;
-        static LdsAttr attr;
+        static LdsLimit attr;
         if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
         hipLaunchKernelGGL(kern, dim3((batch + PC_G - 1) / PC_G), dim3(256), lds, st, P, y, sv, ws + w.dconcat, mask, mstride, grad, batch);
         LAUNCH_CHECK();
@@ -1328,7 +1319,7 @@ static int launch_train_encoder(bool drop, int nblk, const float *P, const CateL
     const size_t lds = Ge::lds_floats * sizeof(float);
     auto k_drop = encoder8_kernel<8, 7, 2>;
     auto k_nodrop = encoder8_kernel<8, 7, 1>;
-    static LdsAttr a_drop, a_nodrop;
+    static LdsLimit a_drop, a_nodrop;
     if (int rc = ensure_lds(a_drop, reinterpret_cast<const void *>(k_drop), lds)) return rc;
     if (int rc = ensure_lds(a_nodrop, reinterpret_cast<const void *>(k_nodrop), lds)) return rc;
     hipLaunchKernelGGL(drop ? k_drop : k_nodrop, dim3(nblk), dim3(256), lds, st, P, e, xt, temb, 1, mask, mstride, concat, B, sv, dm);
@@ -1343,7 +1334,7 @@ static int launch_train_enc_bwd(int nblk, const float *P, const TrainLayout &tl,
     typedef TrbGeom<8, G, 8, 128> Ge;
     const size_t lds = Ge::lds_floats * sizeof(float);
     auto kern = cate_enc_bwd_kernel<8, 7, G, 8, 128>;
-    static LdsAttr attr;
+    static LdsLimit attr;
     if (int rc = ensure_lds(attr, reinterpret_cast<const void *>(kern), lds)) return rc;
     hipLaunchKernelGGL(kern, dim3(nblk), dim3(256), lds, st, P, tl, sv, xt, dconcat, mask, mstride, dm, part, gl, dtau, B);
     LAUNCH_CHECK();

@@ -367,3 +367,9 @@ def test_two_first_calls_leave_the_larger_lds_limit(tmp_path):
     for _ in range(3):
         out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.split()
         assert out == [str(120 * 1024), "0"], out
+
+
+def test_every_lds_limit_is_set_under_the_lock():
+    csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    setting = [f for f in sorted(os.listdir(csrc)) if f.endswith((".hip", ".h")) and "hipFuncSetAttribute(" in open(os.path.join(csrc, f)).read()]
+    assert setting == ["dnag_lds_limit.h"]
