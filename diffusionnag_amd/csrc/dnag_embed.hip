@@ -326,10 +326,11 @@ __global__ __launch_bounds__(512) void embed_join_kernel(const uint32_t *__restr
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 namespace {
+constexpr int64_t JOIN_CLEAR = 1024;   // workgroups behind the join's that clear rows, at most
 struct GradPlan {
     bool few = false, lds = false;
     int64_t per_block = 0;             // few: rows per block; radix sort: list entries per block
-    int nblk = 0, chunk = 0, nchunk = 0, passes = 0;
+    int nblk = 0, chunk = 0, nchunk = 0, passes = 0, jtile = 0;      // jtile: the join's tiles of 256 columns
     size_t part = 0, key[2] = {}, pos[2] = {}, hist = 0, last = 0, bytes = 0;      // offsets into the workspace
 };
 
@@ -351,6 +352,7 @@ GradPlan grad_plan(int64_t rows, int64_t V, int64_t d) {
     p.chunk = 64;                      // fewer pieces, but no fewer waves than eight for each of 256 CUs
     while (p.chunk > 8 && ceil_div(rows, p.chunk) * wide < 4096) p.chunk /= 2;
     p.nchunk = (int)ceil_div(rows, p.chunk);
+    p.jtile = (int)ceil_div(d, 256);
     if (!p.lds) {
         p.per_block = ceil_div(ceil_div(rows, EMB_MAXB), 256) * 256;
         if (p.per_block < 1024) p.per_block = 1024;
@@ -447,13 +449,10 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
     hipLaunchKernelGGL(sum, dim3((unsigned)ceil_div(units, 256 / tpr)), dim3(256), 0, st, key[now], pos[now], rows, g, gs, (uint32_t)V, (int)d, scale, p.chunk, (int)ntile,
                        (T *)out, last, part);
     TOK_TRY(hipGetLastError());
-    // (a chunk's number fits: at least 8 rows each)
-    const int jtile = (int)ceil_div(d, 256);
-    const int64_t joins = p.nchunk * (int64_t)jtile;
-    if (int rc = grid_fits(joins + 1024, 512)) return rc;
-    const int64_t clear = p.passes > 1 ? 0 : V < 1024 ? V : 1024;
+    const int64_t joins = p.nchunk * (int64_t)p.jtile;
+    const int64_t clear = p.passes > 1 ? 0 : V < JOIN_CLEAR ? V : JOIN_CLEAR;
     const EmbFill f = {last, (uint16_t *)out, 0, V, d * (int64_t)(sizeof(T) / 2), (int)joins};
-    hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)(joins + clear)), dim3(512), 0, st, key[now], last, rows, (uint32_t)V, part, p.chunk, jtile, (int)d, scale,
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)(joins + clear)), dim3(512), 0, st, key[now], last, rows, (uint32_t)V, part, p.chunk, p.jtile, (int)d, scale,
                        (T *)out, f);
     TOK_TRY(hipGetLastError());
     return 0;
@@ -496,6 +495,8 @@ extern "C" int dnag_embed_grad(const void *ids, int ids_bytes, int64_t rows, con
         return 0;
     }
     const GradPlan p = grad_plan(rows, num_tokens, dim);
+    // before anything is launched; the join's grid has the most lanes: 512 for 256 columns of a chunk, the sum's one for eight
+    if (!p.few) if (int rc = grid_fits(p.nchunk * (int64_t)p.jtile + JOIN_CLEAR, 512)) return rc;
     if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return dnag_fail(DNAG_E_WORKSPACE, "workspace has %zu bytes, %zu are needed", workspace_bytes, p.bytes);
     return EMB_DISPATCH(grad_t, p, ids, rows, grad, grad_stride, num_tokens, dim, scale, padding_idx, out, (char *)workspace, st);
 }

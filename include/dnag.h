@@ -402,7 +402,8 @@ int dnag_embed_forward(const void *ids, int ids_bytes, int64_t rows, const void 
                        int64_t num_tokens, int64_t dim, int dtype, float scale, void *out, void *stream);
 /* Its gradient: out[v] = scale * sum over t with ids[t] = v of grad[t], in fp32 and in one fixed order (the same bits every
  * time), rounded once to `dtype`.  Every row of out [num_tokens][dim] is written: zeros for tokens that do not occur and for
- * padding_idx (negative: none).  The workspace may be reused as soon as the stream has passed the call. */
+ * padding_idx (negative: none).  With more than 16 tokens rows * ceil(dim / 256) is at most 5.3e8.  The workspace may be
+ * reused as soon as the stream has passed the call. */
 size_t dnag_embed_grad_workspace_bytes(int64_t rows, int64_t num_tokens, int64_t dim);
 int dnag_embed_grad(const void *ids, int ids_bytes, int64_t rows, const void *grad, int64_t grad_stride, int64_t num_tokens,
                     int64_t dim, int dtype, float scale, int64_t padding_idx, void *out, void *workspace, size_t workspace_bytes,

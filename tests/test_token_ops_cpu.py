@@ -373,3 +373,11 @@ def test_every_lds_limit_is_set_under_the_lock():
     csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
     setting = [f for f in sorted(os.listdir(csrc)) if f.endswith((".hip", ".h")) and "hipFuncSetAttribute(" in open(os.path.join(csrc, f)).read()]
     assert setting == ["dnag_lds_limit.h"]
+
+
+@pytest.mark.parametrize("rows,num_tokens,dim", [(0x7fffffff, 1000, 8), (1 << 30, 17, 1), (1 << 28, 70000, 4096), (600_000_000, 1 << 20, 256)])
+def test_embed_grad_refuses_too_many_rows_before_it_launches(rows, num_tokens, dim):
+    """Addresses that are not NULL stand for device memory; a launch would end in another error here, without a device."""
+    P = 4096
+    for dtype in (0, 1, 2):
+        refused(_lib.load().dnag_embed_grad(P, 8, rows, P, dim, num_tokens, dim, dtype, 1.0, -1, P, P, 1 << 62, None), "too many rows")
