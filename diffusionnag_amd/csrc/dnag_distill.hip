@@ -281,38 +281,39 @@ DistillArgs fill(const dnag_distill_args &p) {
     a.scale = mean && !p.row_weight ? 1.0f / (float)p.rows : 1.0f;
     return a;
 }
+int weights(const DistillArgs &a, float *wsum, hipStream_t st) {
+    if (!a.wsum) return 0;
+    hipLaunchKernelGGL(distill_weight_kernel, dim3(1), dim3(1024), 0, st, a.weight, a.rows, wsum);
+    TOK_TRY(hipGetLastError());
+    return 0;
+}
 template <class T, int MODE, int TPR, int NV>
-int launch(const DistillArgs &a, hipStream_t st) {
+int launch(const DistillArgs &a, float *wsum, hipStream_t st) {
     constexpr int NT = TPR <= 64 ? 256 / TPR : 1;
     const int64_t lanes = NV > 0 ? ceil_div(a.V, 8 * NV) : TPR;        // a team above 64 lanes: whole waves, as many as the row fills
     const unsigned threads = TPR <= 64 ? 256 : (unsigned)(ceil_div(lanes, 64) * 64);
     if (int rc = grid_fits(ceil_div(a.rows, NT), threads)) return rc;
+    if (int rc = weights(a, wsum, st)) return rc;      // the call's first launch: nothing is refused behind it
     hipLaunchKernelGGL((distill_kernel<T, TPR, NV, MODE>), dim3((unsigned)ceil_div(a.rows, NT)), dim3(threads), (size_t)NT * a.K * 12, st, a);
     TOK_TRY(hipGetLastError());
     return 0;
 }
 // lanes of a row's team and pieces of eight elements that a lane keeps: the smallest team that holds the row
 template <class T, int MODE>
-int launch_size(const DistillArgs &a, hipStream_t st) {
+int launch_size(const DistillArgs &a, float *wsum, hipStream_t st) {
     const int V = a.V;
-    if (V <= 64 && a.K <= 128) return launch<T, MODE, 8, 1>(a, st);
-    if (V <= 512) return launch<T, MODE, 64, 1>(a, st);
-    if (V <= 2048) return launch<T, MODE, 64, 4>(a, st);
-    if (V <= 8192) return launch<T, MODE, 256, 4>(a, st);
-    if (V <= 32768) return launch<T, MODE, 512, 8>(a, st);
-    if (V <= 65536) return launch<T, MODE, 1024, 8>(a, st);
-    if (sizeof(T) == 2 && V <= 131072) return launch<T, MODE, 1024, sizeof(T) == 2 ? 16 : 0>(a, st);
-    return launch<T, MODE, 1024, 0>(a, st);
+    if (V <= 64 && a.K <= 128) return launch<T, MODE, 8, 1>(a, wsum, st);
+    if (V <= 512) return launch<T, MODE, 64, 1>(a, wsum, st);
+    if (V <= 2048) return launch<T, MODE, 64, 4>(a, wsum, st);
+    if (V <= 8192) return launch<T, MODE, 256, 4>(a, wsum, st);
+    if (V <= 32768) return launch<T, MODE, 512, 8>(a, wsum, st);
+    if (V <= 65536) return launch<T, MODE, 1024, 8>(a, wsum, st);
+    if (sizeof(T) == 2 && V <= 131072) return launch<T, MODE, 1024, sizeof(T) == 2 ? 16 : 0>(a, wsum, st);
+    return launch<T, MODE, 1024, 0>(a, wsum, st);
 }
 template <int MODE>
-int launch_type(int dtype, const DistillArgs &a, hipStream_t st) {
-    return dtype == DNAG_F32 ? launch_size<float, MODE>(a, st) : dtype == DNAG_BF16 ? launch_size<tbf16, MODE>(a, st) : launch_size<tf16, MODE>(a, st);
-}
-int weights(const dnag_distill_args &p, const DistillArgs &a) {
-    if (!a.wsum) return 0;
-    hipLaunchKernelGGL(distill_weight_kernel, dim3(1), dim3(1024), 0, (hipStream_t)p.stream, p.row_weight, p.rows, (float *)p.workspace);
-    TOK_TRY(hipGetLastError());
-    return 0;
+int launch_type(int dtype, const DistillArgs &a, float *wsum, hipStream_t st) {
+    return dtype == DNAG_F32 ? launch_size<float, MODE>(a, wsum, st) : dtype == DNAG_BF16 ? launch_size<tbf16, MODE>(a, wsum, st) : launch_size<tf16, MODE>(a, wsum, st);
 }
 int forward(const dnag_distill_args *p, bool with_grad) {
     if (int rc = check(p)) return rc;
@@ -326,8 +327,8 @@ int forward(const dnag_distill_args *p, bool with_grad) {
     a.row_loss = none ? p->loss : (float *)((char *)p->workspace + w.row_loss);
     a.stats = p->stats;
     a.grad = p->grad;
-    if (int rc = weights(*p, a)) return rc;
-    if (int rc = with_grad ? launch_type<1>(p->dtype, a, st) : launch_type<0>(p->dtype, a, st)) return rc;
+    float *wsum = (float *)p->workspace;
+    if (int rc = with_grad ? launch_type<1>(p->dtype, a, wsum, st) : launch_type<0>(p->dtype, a, wsum, st)) return rc;
     if (!none) {
         hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, st, a.row_loss, p->rows, a.wsum, a.scale, p->loss);
         TOK_TRY(hipGetLastError());
@@ -352,6 +353,5 @@ extern "C" int dnag_distill_backward(const dnag_distill_args *p) {
     a.gout = p->grad_out;
     a.gstep = p->reduction == DNAG_REDUCE_NONE ? 1 : 0;
     a.grad = p->grad;
-    if (int rc = weights(*p, a)) return rc;
-    return launch_type<2>(p->dtype, a, (hipStream_t)p->stream);
+    return launch_type<2>(p->dtype, a, (float *)p->workspace, (hipStream_t)p->stream);
 }

@@ -381,3 +381,14 @@ def test_embed_grad_refuses_too_many_rows_before_it_launches(rows, num_tokens, d
     P = 4096
     for dtype in (0, 1, 2):
         refused(_lib.load().dnag_embed_grad(P, 8, rows, P, dim, num_tokens, dim, dtype, 1.0, -1, P, P, 1 << 62, None), "too many rows")
+
+
+@pytest.mark.parametrize("call", ["dnag_distill_loss", "dnag_distill_loss_grad", "dnag_distill_backward"])
+@pytest.mark.parametrize("rows,vocab", [(0x7fffffff, 1000), (1 << 27, 5000), (1 << 25, 100000)])
+def test_distill_refuses_too_many_rows_before_it_launches(call, rows, vocab):
+    """With row weights and 'mean' the sum of the weights is the first launch; without a device it would end in another error."""
+    P = 4096
+    for dtype in (0, 1, 2):
+        a = _lib.DistillArgsC(rows=rows, vocab=vocab, logits_stride=vocab, k=3, dtype=dtype, ids_bytes=8, reduction=2, temperature=1.0, logits=P, teacher_ids=P,
+                              teacher_logits=P, row_weight=P, loss=P, stats=P, grad_out=P, grad=P, workspace=P, workspace_bytes=1 << 60)
+        refused(getattr(_lib.load(), call)(C.byref(a)), "too many rows")
