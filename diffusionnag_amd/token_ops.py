@@ -205,6 +205,8 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
         raise ValueError(f"grad {tuple(grad.shape)} does not match ids {tuple(ids.shape)}")
     if num_tokens < 1 or grad.shape[-1] < 1:
         raise ValueError(f"num_tokens={num_tokens}, dim={grad.shape[-1]}: both must be positive")
+    if padding_idx is not None and not 0 <= padding_idx < num_tokens:
+        raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {num_tokens - 1}")
     code = _dtype(grad, "grad")
     _no_tangents(grad)
     index = _device(grad, ids)

@@ -392,3 +392,10 @@ def test_distill_refuses_too_many_rows_before_it_launches(call, rows, vocab):
         a = _lib.DistillArgsC(rows=rows, vocab=vocab, logits_stride=vocab, k=3, dtype=dtype, ids_bytes=8, reduction=2, temperature=1.0, logits=P, teacher_ids=P,
                               teacher_logits=P, row_weight=P, loss=P, stats=P, grad_out=P, grad=P, workspace=P, workspace_bytes=1 << 60)
         refused(getattr(_lib.load(), call)(C.byref(a)), "too many rows")
+
+
+@pytest.mark.parametrize("padding_idx", [-1, 4, 10 ** 20])
+def test_embed_grad_refuses_the_padding_that_the_lookup_refuses(padding_idx):
+    """-1 is torch's name for the last token; taken as none, its row would get a gradient."""
+    with pytest.raises(ValueError, match="padding_idx"):
+        ops.embed_tokens_grad(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 4, padding_idx=padding_idx)
