@@ -844,3 +844,64 @@ def test_captured_training_step_through_autograd():
         with pytest.raises(RuntimeError, match="eager autograd graph"):
             ops.embed_tokens(ids, w)
     del alive
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# workgroups that take several rows, runs or column tiles
+# ---------------------------------------------------------------------------------------------------------------
+F, B16, H16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("rows,d,groups,types,kind", [
+    (700, 4100, 1, (B16, B16, B16), "rms"), (600, 8192, 2, (B16, B16, F), "rms"), (1200, 4104, 600, (H16, H16, H16), "rms"),         # the next row asked for ahead
+    (700, 4100, 1, (F, F, F), "layer"), (700, 4100, 7, (F, B16, B16), "rms"), (600, 5000, 2, (B16, B16, B16), "layer"),              # not ahead
+    (3000, 640, 3, (B16, B16, F), "rms"), (3000, 640, 3, (F, F, F), "layer"), (1100, 520, 1100, (F, B16, B16), "layer"), (4000, 1100, 2, (B16, B16, B16), "rms"),
+    (1300, 2100, 5, (H16, H16, F), "layer"), (600, 8200, 1, (B16, B16, B16), "rms"), (600, 8200, 300, (F, F, F), "layer"), (520, 16384, 1, (F, B16, B16), "rms")])
+def test_block_norms_many_rows_of_a_workgroup(rows, d, groups, types, kind):
+    """Above 512 columns a team is the workgroup (or one of two halves of it): more rows than workgroups, so that each goes through several rows of
+    one gate (700 of 4100: three), or through several gates (1100 gates of 520: two for some)."""
+    g = gen(rows + d)
+    check_norms(norm_inputs(g, rows, d, groups, *types, kind), kind, 0.9, True, g)
+
+
+@pytest.mark.parametrize("rows,V,d", [(8200, 300, 2100), (9000, 3000, 520), (8200, 20000, 2100), (60000, 300, 2100), (270000, 20000, 24)])
+@pytest.mark.parametrize("hot", [False, True])
+def test_embed_grad_wide_rows_and_long_lists(rows, V, d, hot):
+    """The sorted list with teams of several widths, several column tiles, zero rows longer than a workgroup clears at once, and chunks of 8 to 64
+    entries.  Sums in 64 bits by index_add_."""
+    g = gen(rows + V + d + hot)
+    dtype = DTYPES[(rows // 1000 + hot) % 3]
+    grad, ids = rnd(g, rows, d, dtype=dtype), some_ids(g, rows, V, hot)
+    at = torch.where((ids >= 0) & (ids < V), ids, V)
+    n = torch.bincount(at, minlength=V + 1)[:V, None].double()
+    want = torch.zeros(V + 1, d, dtype=torch.float64).index_add_(0, at, grad.double())[:V] * 1.5
+    mag = torch.zeros(V + 1, d, dtype=torch.float64).index_add_(0, at, grad.double().abs())[:V] * 1.5
+    got = ops.embed_tokens_grad(dev(grad), dev(ids), V, scale=1.5)
+    within(got, want, (n + 2) * U32 * mag, f"{dtype}")
+    assert not got[dev((n == 0).squeeze(1))].any()
+    assert torch.equal(got, ops.embed_tokens_grad(dev(grad), dev(ids.int()), V, scale=1.5)), "the same inputs gave other bits"
+
+
+def test_gates_of_positions():
+    """A gate for each position of every sequence is expanded to the shape of x; its gradient comes back through the expansion."""
+    g = gen(8)
+    x, y, gate = rnd(g, 5, 6, 70), rnd(g, 5, 6, 70), rnd(g, 1, 6, 70)
+    cx, ch = rnd(g, 5, 6, 70), rnd(g, 5, 6, 70)
+    flat = norm_inputs(g, 30, 70, 30, F, F, F, "rms")
+    flat.update(x=x.reshape(30, 70), y=y.reshape(30, 70), gate=gate.expand(5, 6, 70).reshape(30, 70))
+    tol = norm_tolerances(flat, "rms", 1e-6, 1.0, True, cx.reshape(30, 70), ch.reshape(30, 70))
+    T = {n: None if v is None else v.double() for n, v in flat.items()}
+    rows_gate = T["gate"].clone().requires_grad_(True)
+    xn, h = R.block_norms({**T, "gate": rows_gate}, 1.0, "rms", 1e-6, True)
+    (each,) = torch.autograd.grad((xn.reshape(5, 6, 70) * cx).sum() + (h.reshape(5, 6, 70) * ch).sum(), rows_gate)
+    each = each.reshape(5, 6, 70)
+    leaf = dev(gate).requires_grad_(True)
+    x_new, got_h = ops.block_norms(dev(x), dev(y), gate=leaf.expand(5, 6, 70), post_weight=dev(flat["post_weight"]), pre_weight=dev(flat["pre_weight"]))
+    within(x_new.reshape(30, 70), xn.detach(), tol["x_new"], "x_new")
+    within(got_h.reshape(30, 70), h.detach(), tol["h"], "h")
+    (got,) = torch.autograd.grad([x_new, got_h], leaf, [dev(cx), dev(ch)])
+    slack = tol["gate"].reshape(5, 6, 70).sum(0) + 6 * U32 * each.abs().sum(0)             # each one rounded to fp32, then five of them added
+    within(got[0], each.sum(0), slack, "gradient of the gate")
+    for bad in (dev(gate), dev(gate)[0]):
+        with pytest.raises(ValueError, match="gate"):
+            ops.block_norms(dev(x), dev(y), gate=bad)
