@@ -13,7 +13,11 @@
 #include "dnag_token_common.h"
 
 #define EMB_FEW 16              // 16 rows of 64 columns for each of 32 teams: 128 KB of LDS
-#define EMB_SORT_LDS 8192       // (token, position) pairs of 8 bytes: 64 KB of LDS
+// Rows that one workgroup sorts in LDS, three launches in all instead of four to eight: its time grows with the rows, the radix sort's with the
+// passes over the tokens' digits.  In us, this and the radix sort, bf16: 1024 rows over 100 x 64 24 and 18, 300 x 512 23 and 26, 32000 x 512
+// 34 and 44, 100000 x 64 54 and 85; 2048 rows 30 and 18, 29 and 27, 41 and 43, 60 and 80; 4096 rows 46 and 19, 46 and 29, 59 and 43,
+// 77 and 78.
+#define EMB_SORT_LDS 2048
 
 template <class I> __device__ __forceinline__ uint32_t emb_key(const I *ids, size_t t, int64_t V, int64_t pad) {
     const int64_t v = (int64_t)ids[t];
@@ -417,11 +421,8 @@ int grad_t(const GradPlan &p, const void *ids, int64_t rows, const void *grad, i
     if (p.lds) {
         int n2 = 2;
         while (n2 < rows) n2 *= 2;
-        auto kern = embed_sort_lds_kernel<I>;
-        static LdsLimit limit;
-        TOK_TRY(limit.allow((const void *)kern, (size_t)n2 * 8));
         const unsigned zero = (unsigned)(ceil_div(V, 4096) < 256 ? ceil_div(V, 4096) : 256);
-        hipLaunchKernelGGL(kern, dim3(1 + zero), dim3(1024), (size_t)n2 * 8, st, id, (int)rows, n2, V, pad, key[0], pos[0], last);
+        hipLaunchKernelGGL((embed_sort_lds_kernel<I>), dim3(1 + zero), dim3(1024), (size_t)n2 * 8, st, id, (int)rows, n2, V, pad, key[0], pos[0], last);
         TOK_TRY(hipGetLastError());
     } else {
         // The first scatter marks the tokens that occur; from then on 512 workgroups more per launch clear the others' rows

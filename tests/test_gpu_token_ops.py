@@ -905,3 +905,20 @@ def test_gates_of_positions():
     for bad in (dev(gate), dev(gate)[0]):
         with pytest.raises(ValueError, match="gate"):
             ops.block_norms(dev(x), dev(y), gate=bad)
+
+
+@pytest.mark.parametrize("rows", [2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("V,d", [(17, 40), (255, 8), (300, 70), (70000, 3)])
+def test_embed_grad_on_both_sides_of_the_sorts_border(rows, V, d):
+    """Lists of up to 2048 entries are sorted by one workgroup, longer ones by digits; the sums run in the same order, so a list that grows by dropped
+    rows over the border gives the same bits."""
+    g = gen(rows + V + d)
+    grad, ids = rnd(g, rows, d), some_ids(g, rows, V, True)
+    want, mag, n = R.embed_grad(ids, grad, V, 1.5, 3)
+    got = ops.embed_tokens_grad(dev(grad), dev(ids), V, scale=1.5, padding_idx=3)
+    within(got, want, (n + 2) * U32 * mag, "sum")
+    assert not got[dev((n == 0).squeeze(1))].any()
+    if rows <= 2048:                                   # (as many entries for a team: 8 up to 32768 rows)
+        more = ops.embed_tokens_grad(torch.cat([dev(grad), torch.full((3000, d), float("nan"), device=DEV)]), torch.cat([dev(ids), torch.full((3000,), -1, device=DEV)]), V,
+                                     scale=1.5, padding_idx=3)
+        assert torch.equal(more, got)
