@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 from torch._ops import mode_stack_state_for_pre_dispatch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -33,7 +34,10 @@ _IDS = {torch.int32: 4, torch.int64: 8}
 
 _MOST = 1.7976931348623157e308
 
-_pre_dispatch_modes = mode_stack_state_for_pre_dispatch()
+# read by every call, so bound once; [0] of the modes before dispatch is a recording one (or None)
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_pre_dispatch_modes = vars(mode_stack_state_for_pre_dispatch()).get("_ModeStackStateForPreDispatch__infra_modes", (None,))
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 Number = Union[int, float]
 
@@ -63,8 +67,8 @@ def _device(*tensors: Optional[torch.Tensor]) -> int:
 
 def _launch(fn, index: int, what: str, *args) -> None:
     """``fn(*args, stream)`` on the device's current stream, with the device current for the call."""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    before = torch._C._cuda_getDevice()
+    stream = _raw_stream(index)
+    before = _current_device()
     if before == index:
         rc = fn(*args, stream)
     else:
@@ -104,23 +108,19 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _not_recorded() -> None:
-    """Refuses to be recorded by torch.jit.trace and make_fx: they would see the allocation of the result and not the launch that fills
-    it, and the recorded program would return memory as it is.  (Three reads of thread-local state, 0.4 us.)"""
-    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None) \
-            or _pre_dispatch_modes.get(0) is not None:         # 0: the recording mode's place
+def _plain(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses to be recorded or differentiated in ways that would pass the launch over without an error (0.2 us where nothing of the kind goes on).
+
+    torch.jit.trace and make_fx would record the allocation of the result and not the launch that fills it: the recorded program would return
+    memory as it is.  Dual tensors of forward-mode differentiation (``tensors``: the differentiable arguments) have requires_grad False; the
+    result would have no tangent, which counts as a derivative of zero."""
+    if (_is_tracing() or _dispatch_modes() or _pre_dispatch_modes[0] is not None) and (_is_tracing() or get_proxy_mode() is not None):
         raise RuntimeError("the token operators cannot be recorded by torch.jit.trace or make_fx: call them, or capture the calls into a HIP graph")
-
-
-def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
-    """Refuses dual tensors of forward-mode differentiation: the operators have no tangents, and a result without one would count as
-    a derivative of zero.  (Outside a dual level there are none: 0.1 us.)"""
-    if forward_ad._current_level < 0:
-        return
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError("the token operators have no forward-mode derivative: an argument carries a tangent (differentiate backward, or "
-                               "take the primal out with torch.autograd.forward_ad.unpack_dual)")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the token operators have no forward-mode derivative: an argument carries a tangent (differentiate backward, or "
+                                   "take the primal out with torch.autograd.forward_ad.unpack_dual)")
 
 
 def _leaf_mark(*tensors: Optional[torch.Tensor]) -> None:
@@ -179,11 +179,10 @@ def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: Number = 1.0
 
     ``ids`` outside ``0 .. len(weight) - 1`` (the -1 or -100 of a padded batch, another shard's tokens) give rows of zeros and
     take no part in the gradient; ``padding_idx`` is looked up but takes no part in the gradient (as in torch)."""
-    _not_recorded()
+    _plain(weight)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [num_tokens, dim], got {tuple(weight.shape)}")
     _dtype(weight, "weight")
-    _no_tangents(weight)
     ids = _check_ids(ids)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {weight.shape[0] - 1}")
@@ -198,7 +197,7 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
                       padding_idx: Optional[int] = None) -> torch.Tensor:
     """Gradient of ``embed_tokens`` with respect to ``weight`` ([num_tokens, d], the type of ``grad``): the rows of ``grad``
     summed by token in float32, in the order of the tokens' positions, the same bits every time."""
-    _not_recorded()
+    _plain(grad)
     lib = _lib.load()
     ids = _check_ids(ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
@@ -208,7 +207,6 @@ def embed_tokens_grad(grad: torch.Tensor, ids: torch.Tensor, num_tokens: int, *,
     if padding_idx is not None and not 0 <= padding_idx < num_tokens:
         raise ValueError(f"padding_idx={padding_idx} is outside 0 .. {num_tokens - 1}")
     code = _dtype(grad, "grad")
-    _no_tangents(grad)
     index = _device(grad, ids)
     g, stride = _rows2d(grad)
     rows, d = g.shape
@@ -410,8 +408,7 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     G-th part of the rows of ``x``, in order, uses one.  A gate that broadcasting would repeat over a leading dimension ([1, N, d] or [N, d] beside
     [B, N, d]) is refused: expand it to the shape of ``x``.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
-    _not_recorded()
-    _no_tangents(*tensors)
+    _plain(*tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _leaf_mark(*tensors)
         out = _BlockNorms.apply(*tensors, residual_scale, norm, eps, pre, dtype)
@@ -429,8 +426,7 @@ def block_norms_grad(grad_x: Optional[torch.Tensor], grad_h: Optional[torch.Tens
                      dtype: Optional[torch.dtype] = None) -> BlockNormsGrad:
     """Gradients of ``block_norms`` (same arguments) for ``grad_x`` and ``grad_h``, the gradients of ``x_new`` and ``h`` (None: zero).
     Nothing of the forward pass but its inputs is needed.  Sums over rows run in one fixed order."""
-    _not_recorded()
-    _no_tangents(grad_x, grad_h, x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
+    _plain(grad_x, grad_h, x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     seam = _Seam(x, y, gate, residual_scale, post_weight, post_bias, pre_weight, pre_bias, norm, eps, pre, dtype)
     return seam.backward(grad_x, grad_h, _SMALL)
 
@@ -519,10 +515,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     or their type's lowest value have no probability (a row of nothing but lowest values: one and the same probability).
     ``temperature`` is 1e-6 to 1e6 (float16 logits: from 0.1 on).  No gradient reaches the
     teacher or the weights: they must not require one."""
-    _not_recorded()
+    _plain(logits, teacher_logits, row_weight)
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
         raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")
-    _no_tangents(logits, teacher_logits, row_weight)
     if logits.requires_grad and torch.is_grad_enabled():
         _leaf_mark(logits)
         return _DistillLoss.apply(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction)
@@ -533,8 +528,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
                           row_weight: Optional[torch.Tensor] = None, reduction: str = "mean"):
     """``distill_loss`` and its gradient with respect to ``logits`` (for an upstream gradient of 1) in one pass over the logits: two
     thirds of the memory traffic of the loss followed by its backward pass.  Returns ``(loss, grad)``."""
-    _not_recorded()
-    _no_tangents(logits, teacher_logits, row_weight)
+    _plain(logits, teacher_logits, row_weight)
     loss, _, grad = _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss(grad=True)
     return loss, grad
 
@@ -552,7 +546,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[N
     index.  The token is the first one, in index order, whose running sum of kept probability exceeds ``u`` times the total.
     NaN and -inf are never drawn; a row of nothing else gives -1.  Each setting is a number, or a tensor with a value per
     row (float32; int32 for ``top_k``).  The same inputs give the same tokens, whatever else runs.  vocab <= 2^20."""
-    _not_recorded()
+    _plain()                                           # tokens have no derivative
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
     lead = logits.shape[:-1]

@@ -399,3 +399,12 @@ def test_embed_grad_refuses_the_padding_that_the_lookup_refuses(padding_idx):
     """-1 is torch's name for the last token; taken as none, its row would get a gradient."""
     with pytest.raises(ValueError, match="padding_idx"):
         ops.embed_tokens_grad(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 4, padding_idx=padding_idx)
+
+
+def test_other_dispatch_modes_are_no_recording(monkeypatch):
+    """Counting or printing modes only look on: the calls work inside them."""
+    from torch.utils.flop_counter import FlopCounterMode
+    monkeypatch.setattr(ops, "_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_launch", lambda *a: None)
+    with FlopCounterMode(display=False):
+        assert ops.embed_tokens(IDS, torch.ones(4, 8)).shape == (3, 8) and ops.sample_tokens(torch.ones(3, 8), torch.zeros(3)).shape == (3,)
