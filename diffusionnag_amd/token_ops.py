@@ -410,7 +410,6 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     _plain(*tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        _device(*tensors)
         _leaf_mark(*tensors)
         out = _BlockNorms.apply(*tensors, residual_scale, norm, eps, pre, dtype)
         if y is None:
@@ -520,7 +519,6 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
         raise ValueError("distill_loss has no gradient for teacher_logits and row_weight: detach them")
     if logits.requires_grad and torch.is_grad_enabled():
-        _device(logits, teacher_ids, teacher_logits, row_weight)
         _leaf_mark(logits)
         return _DistillLoss.apply(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction)
     return _Distill(logits, teacher_ids, teacher_logits, temperature, row_weight, reduction).loss()[0]

@@ -408,10 +408,3 @@ def test_other_dispatch_modes_are_no_recording(monkeypatch):
     monkeypatch.setattr(ops, "_launch", lambda *a: None)
     with FlopCounterMode(display=False):
         assert ops.embed_tokens(IDS, torch.ones(4, 8)).shape == (3, 8) and ops.sample_tokens(torch.ones(3, 8), torch.zeros(3)).shape == (3,)
-
-
-@pytest.mark.parametrize("what", [w for w in DIFFERENTIABLE if w not in ("distillation teacher", "distillation weight")])
-def test_cpu_tensors_are_refused_with_a_gradient_too(what):
-    shape, call = DIFFERENTIABLE[what]
-    with pytest.raises(RuntimeError, match="no CPU fallback"):
-        call(torch.ones(shape, requires_grad=True))
