@@ -7,8 +7,9 @@
 //   The backward pass reads x and y again and recomputes x' in fp32: as many bytes as reading a saved x', without its rounding.
 // Bound by HBM: four rows per row forward, six or seven backward.  A team of TPR lanes holds a row in registers, eight
 // columns per lane (and twice that above 8192 columns), so every value is read once; statistics are fp32 and two-pass
-// (mean first) for LayerNorm.  16384 x 4096 bf16 forward: 102 us, 5.3 TB/s; backward 16384 x 2048 with fp32 rows beside bf16: 137 us,
-// 4.4 TB/s.  Rows of more than 8192 columns keep their pieces partly in scratch in the backward pass: 2048 x 16384 bf16 takes 354 us.
+// (mean first) for LayerNorm.  16384 x 4096 bf16 forward: 99 us, 5.4 TB/s; backward 16384 x 2048 with fp32 rows beside bf16: 135 us,
+// 4.5 TB/s.  Rows of more than 8192 columns keep their pieces and sums partly in scratch in the backward pass (the 128 registers of a lane
+// of 1024 do not hold two pieces of each; 400 to 750 bytes a lane): 2048 x 16384 bf16 takes 372 us, its 403 MB at the copy rate 79.
 // Gradients of the weights and of shared gates are summed by every block over its own rows in
 // registers, then over blocks in block order by a second launch: no atomics, the same bits every time.
 #include "dnag_token_common.h"
@@ -371,7 +372,9 @@ BnPlan grad_plan(const dnag_block_norms_args &p) {
     q.nt = q.tpr <= 64 ? 256 / q.tpr : 1;
     q.na = p.layer_norm ? 4 : 2;
     const int64_t G = p.gate_rows, rpg = p.rows / G;
-    // as many blocks as the chip holds at a time, or twice that: fewer partial sums than with a block per row
+    // as many blocks as the chip holds at a time, or twice that: fewer partial sums than with a block per row.  Half of them, these and
+    // twice as many, us, bf16: 65536 x 64 26, 22, 27; 65536 x 256 75, 49, 55; 32768 x 512 80, 52, 58; 16384 x 1024 101, 61, 53; 16384 x 2048
+    // 128, 96, 102; 16384 x 4096 289, 197, 199; 8192 x 8192 378, 211, 224; 2048 x 16384 565, 345, 380; 1024 x 4096 29, 26, 34
     const int64_t target = q.tpr <= 64 || q.tpr == 512 ? 512 : q.tpr > 512 ? 256 : 1024;
     q.S = 1;
     if (rpg >= q.nt) {

@@ -12,7 +12,10 @@
 //     chunk order and writes the zero rows of the tokens that do not occur.
 #include "dnag_token_common.h"
 
-#define EMB_FEW 16              // 16 rows of 64 columns for each of 32 teams: 128 KB of LDS
+// Tokens whose rows of 64 columns are kept for each of 32 teams: 8 KB of LDS a token, 128 KB at 16.  In us, this and the sorted list, 32768
+// rows: 12 x 64 fp32 8 and 23, 16 x 64 9 and 23, 9 x 1024 bf16 23 and 36, 16 x 1024 38 and 36; with room for 18 (144 KB), 18 x 64 9 and 22,
+// 18 x 1024 40 and 35: wide rows are better sorted from 16 on, narrow ones not before the LDS ends.
+#define EMB_FEW 16
 // Rows that one workgroup sorts in LDS, three launches in all instead of four to eight: its time grows with the rows, the radix sort's with the
 // passes over the tokens' digits.  In us, this and the radix sort, bf16: 1024 rows over 100 x 64 24 and 18, 300 x 512 23 and 26, 32000 x 512
 // 34 and 44, 100000 x 64 54 and 85; 2048 rows 30 and 18, 29 and 27, 41 and 43, 60 and 80; 4096 rows 46 and 19, 46 and 29, 59 and 43,
@@ -152,6 +155,8 @@ __device__ __forceinline__ void emb_fill(const EmbFill &f) {
 
 // Stable radix sort, digits of eight bits.  A block owns a contiguous range of the list and each of its four waves a
 // contiguous quarter; at most EMB_MAXB blocks, so that every block sums the others' histograms by itself (no scan launch).
+// With 64, 128 and 256 of them, us for the whole gradient over 32000 x 64 bf16: 131072 rows 60, 58, 58; 270000 rows 98, 86, 85; 1000000 rows 222,
+// 164, 139.  Up to 131072 rows a block has at least 1024 and the number makes no difference.
 #define EMB_MAXB 128
 template <class I>
 __device__ __forceinline__ uint32_t emb_pass_key(const I *ids, const uint32_t *kin, int64_t i, int64_t V, int64_t pad) {
@@ -231,9 +236,9 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I *__restrict_
     }
 }
 
-// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` (8 to 64, at most TPR) entries.  The lanes fetch the
+// Sums over the sorted list: a team of TPR lanes (TPR * 8 columns) walks `chunk` (8 to 64) entries.  The lanes fetch TPR of the
 // entries at once, one each, so that the rows' addresses are known before the first row is asked for; eight rows are
-// under way at a time (fetching four entries, then their rows, in turn: 94 us for 32768 x 2048 bf16; this: 55, 2.4 TB/s of the
+// under way at a time (fetching four entries, then their rows, in turn: 94 us for 32768 x 2048 bf16; this: 58, 2.3 TB/s of the
 // gradient's rows).
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t rows,

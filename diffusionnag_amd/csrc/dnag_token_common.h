@@ -1,4 +1,4 @@
-// What the token operators' kernels share (dnag_tokens.hip): element types, eight-element pieces of a row, sums and maxima
+// What the token operators' kernels share (dnag_embed, dnag_block_norms, dnag_distill, dnag_sample .hip): element types, eight-element pieces of a row, sums and maxima
 // over the lanes that hold one row, the launch helpers and the error path.
 #pragma once
 #include <hip/hip_runtime.h>

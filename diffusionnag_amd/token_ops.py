@@ -11,7 +11,8 @@ contiguous last dimension are read in place, others are copied first; outputs ar
 allocator and belong to the call (also under graph capture).  The first three are differentiable through ``torch.autograd``;
 ``embed_tokens_grad``, ``block_norms_grad`` and ``distill_loss_and_grad`` give the same gradients without it, which is also how to
 capture a training step into a graph: a backward pass of ``torch.autograd`` that is captured while an eager graph of the
-same leaves is alive ends the process inside torch, so the differentiable calls raise there.  There is no forward-mode
+same leaves is alive ends the process inside torch, so the differentiable calls raise there for leaves that one of them was given in
+that graph (a graph that only other operations made is not seen).  There is no forward-mode
 derivative: arguments that carry a tangent are refused.  So are torch.jit.trace and make_fx, which would record an empty result;
 torch.compile breaks its graph around the calls.
 Element types: float32, bfloat16, float16.  All sums and statistics are float32 or wider; results are rounded once.
@@ -406,7 +407,8 @@ def block_norms(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Opti
     ``h`` (default: that of ``x``); ``pre=False`` the exit of the last one: ``(x_new, None)``.  ``h`` is computed from
     the unrounded ``x_new``.  ``gate`` has G rows ([d], [B, 1, d], the shape of ``x``, a list [G, d], ...): every
     G-th part of the rows of ``x``, in order, uses one.  A gate that broadcasting would repeat over a leading dimension ([1, N, d] or [N, d] beside
-    [B, N, d]) is refused: expand it to the shape of ``x``.  Weights and gate have the branch's type or float32.  1 <= d <= 16384."""
+    [B, N, d]) is refused: expand it to the shape of ``x``.  Weights and gate have the branch's type or float32.  1 <= d <= 16384.  Squares are
+    summed in float32: magnitudes up to 1e17."""
     tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
     _plain(*tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
@@ -513,7 +515,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     matter, NaN included.  A row without entries counts 0.  ``reduction``: 'mean' over the positive weights (over all rows
     without weights; 0 where there are none), 'sum', or 'none' (weighted loss of each row).  float32.  ``logits`` masked with -inf
     or their type's lowest value have no probability (a row of nothing but lowest values: one and the same probability).
-    ``temperature`` is 1e-6 to 1e6 (float16 logits: from 0.1 on).  No gradient reaches the
+    ``temperature`` is 1e-6 to 1e6 (float16 logits: from 0.1 on); a row's loss is a difference of float32 logarithms, off by a few
+    1e-6 ``temperature``^2 however small it is.  No gradient reaches the
     teacher or the weights: they must not require one."""
     _plain(logits, teacher_logits, row_weight)
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
