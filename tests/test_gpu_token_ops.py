@@ -922,3 +922,17 @@ def test_embed_grad_on_both_sides_of_the_sorts_border(rows, V, d):
         more = ops.embed_tokens_grad(torch.cat([dev(grad), torch.full((3000, d), float("nan"), device=DEV)]), torch.cat([dev(ids), torch.full((3000,), -1, device=DEV)]), V,
                                      scale=1.5, padding_idx=3)
         assert torch.equal(more, got)
+
+
+def test_compiled_callers():
+    """torch.compile breaks its graph around the calls: the same results and gradients as without it."""
+    s = call_inputs(3)
+    w, g = s["w"].requires_grad_(True), s["y"][0]
+
+    def f(ids, w, y):
+        x, h = ops.block_norms(ops.embed_tokens(ids, w, scale=2.0) * 1.5, y + 0.0, pre_weight=g)
+        loss = ops.distill_loss(h * 2, s["tids"], s["tl"], row_weight=s["rw"])
+        return loss, x, ops.sample_tokens(h.detach() * 3, s["rw"], top_k=5)
+    want, got = f(s["ids"], w, s["y"]), torch.compile(f, backend="eager")(s["ids"], w, s["y"])
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert torch.equal(*(torch.autograd.grad(o[0], w)[0] for o in (want, got)))
